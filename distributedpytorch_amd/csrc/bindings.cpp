@@ -1059,6 +1059,7 @@ Tensor mul_f32(const Tensor& a, const Tensor& b) {
 }  // namespace
 
 void bind_transformer(pybind11::module_& m);  // bindings_tfm.cpp
+void bind_lm(pybind11::module_& m);           // bindings_lm.cpp
 void bind_rccl(pybind11::module_& m);         // rccl_comm.cpp
 void bind_peer(pybind11::module_& m);         // peer_comm.cpp
 
@@ -1169,6 +1170,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("set_attention_fwd_pipe", [](bool on) { dpa::set_attention_fwd_pipe(on ? 1 : 0); });
     m.def("wide_gemm_min_tiles", []() { return (int64_t)dpa::wide_gemm_min_tiles(); });
     bind_transformer(m);
+    bind_lm(m);
     bind_rccl(m);
     bind_peer(m);
 }

@@ -1,0 +1,259 @@
+// Bindings for the language-model kernels: attention with score modifiers, head norms with rotation, the scaled token
+// embedding and the distillation loss.  The Python side (ops/attend.py, ops/heads.py, ops/embed.py, ops/distill.py) states
+// what a call may be; the checks here are what the kernels' addressing relies on.
+#include <torch/extension.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include "kernels.h"
+
+namespace {
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+inline hipStream_t cur_stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
+
+#define CHECK_ON(t, like) TORCH_CHECK((t).is_cuda() && (t).device() == (like).device(), #t " must be on " #like "'s GPU")
+#define CHECK_FLAT(t, like, type) do { CHECK_ON(t, like); TORCH_CHECK((t).is_contiguous(), #t " must be contiguous"); \
+                                       TORCH_CHECK((t).scalar_type() == (type), #t ": wrong type"); } while (0)
+inline bool on16(const Tensor& t) { return ((uintptr_t)t.data_ptr()) % 16 == 0; }
+#define CHECK_FLAT16(t, like, type) do { CHECK_FLAT(t, like, type); TORCH_CHECK(on16(t), #t " must be 16-byte aligned"); } while (0)
+
+// ---------------------------------------------------------------- attention
+// element stride of axis i (0 where the axis has one entry), in whole 16-byte steps
+long row_stride(const Tensor& t, int i) {
+    if (t.size(i) <= 1) return 0;
+    TORCH_CHECK(t.stride(i) % 8 == 0 && t.stride(i) >= 0, "attend: rows must be 16-byte aligned");
+    return (long)t.stride(i);
+}
+
+dpa::AttendArgs attend_args(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
+                            const OptTensor& documents, const OptTensor& prefix) {
+    for (const Tensor* t : {&q, &k, &v}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->dim() == 4 && t->scalar_type() == at::kBFloat16, "attend: q, k, v must be bf16 [B,T,H,D] on one GPU");
+        TORCH_CHECK(t->size(3) == 1 || t->stride(3) == 1, "attend: the last axis must be contiguous");
+        TORCH_CHECK(on16(*t), "attend: 16-byte alignment");
+    }
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(2);
+    TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(1) == T && k.size(3) == D, "attend: shapes");
+    TORCH_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && D >= 8 && D % 8 == 0 && D <= 128, "attend: heads");
+    TORCH_CHECK(B <= 65535 && T <= (1 << 22) && Hq <= 65535, "attend: oversized problem");
+    TORCH_CHECK(scale > 1e-12 && scale < 1e12 && softcap >= 0.0 && softcap < 1e12, "attend: scale, softcap");
+    dpa::AttendArgs a{};
+    a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+    a.qb = row_stride(q, 0); a.qt = row_stride(q, 1); a.qh = row_stride(q, 2);
+    a.kb = row_stride(k, 0); a.kt = row_stride(k, 1); a.kh = row_stride(k, 2);
+    a.vb = row_stride(v, 0); a.vt = row_stride(v, 1); a.vh = row_stride(v, 2);
+    if (slopes.has_value()) {
+        CHECK_FLAT((*slopes), q, at::kFloat);
+        TORCH_CHECK(slopes->numel() == Hq, "attend: slopes");
+        a.slopes = slopes->data_ptr<float>();
+    }
+    if (documents.has_value()) {
+        CHECK_FLAT((*documents), q, at::kInt);
+        TORCH_CHECK(documents->numel() == B * T, "attend: documents");
+        a.docs = documents->data_ptr<int>();
+    }
+    if (prefix.has_value()) {
+        CHECK_FLAT((*prefix), q, at::kInt);
+        TORCH_CHECK(prefix->numel() == B, "attend: prefix");
+        a.prefix = prefix->data_ptr<int>();
+    }
+    a.B = (int)B; a.T = (int)T; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.D = (int)D; a.causal = causal;
+    a.scale = (float)scale; a.softcap = (float)softcap;
+    return a;
+}
+
+// -> out [B,T,Hq,D], lse2 [B,Hq,T], ranges (undefined without documents)
+std::vector<Tensor> attend_fwd(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
+                               const OptTensor& documents, const OptTensor& prefix) {
+    dpa::AttendArgs a = attend_args(q, k, v, causal, scale, softcap, slopes, documents, prefix);
+    Guard guard(q.device());
+    Tensor out = torch::empty(q.sizes(), q.options());
+    Tensor lse2 = torch::empty({a.B, a.Hq, a.T}, q.options().dtype(at::kFloat));
+    Tensor ranges;
+    if (out.numel() == 0) return {out, lse2, ranges};
+    if (a.docs != nullptr) {
+        ranges = torch::empty({a.B, (a.T + 63) / 64, 4}, q.options().dtype(at::kInt));
+        dpa::attend_doc_ranges(a.docs, ranges.data_ptr(), a.B, a.T, cur_stream());
+        a.ranges = (const int4*)ranges.data_ptr();
+    }
+    dpa::attend_fwd(a, out.data_ptr(), lse2.data_ptr<float>(), cur_stream());
+    return {out, lse2, ranges};
+}
+
+// -> dq, dk, dv, contiguous
+std::vector<Tensor> attend_bwd(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
+                               const OptTensor& documents, const OptTensor& prefix, const OptTensor& ranges, const Tensor& out, const Tensor& dout,
+                               const Tensor& lse2) {
+    dpa::AttendArgs a = attend_args(q, k, v, causal, scale, softcap, slopes, documents, prefix);
+    CHECK_FLAT16(out, q, at::kBFloat16); CHECK_FLAT16(dout, q, at::kBFloat16); CHECK_FLAT(lse2, q, at::kFloat);
+    TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes() && lse2.numel() == (int64_t)a.B * a.Hq * a.T, "attend_bwd: shapes");
+    Guard guard(q.device());
+    Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), q.options()), dv = torch::empty(k.sizes(), q.options());
+    if (out.numel() == 0) return {dq, dk, dv};
+    if (a.docs != nullptr) {
+        TORCH_CHECK(ranges.has_value() && ranges->numel() == (int64_t)a.B * ((a.T + 63) / 64) * 4, "attend_bwd: ranges");
+        CHECK_FLAT16((*ranges), q, at::kInt);
+        a.ranges = (const int4*)ranges->data_ptr();
+    }
+    Tensor delta = torch::empty_like(lse2);
+    dpa::attend_bwd(a, out.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                    cur_stream());
+    return {dq, dk, dv};
+}
+
+// ---------------------------------------------------------------- head norms and rotation
+dpa::HeadsArgs heads_args(const Tensor& qkv, int64_t Hq, int64_t Hkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& inv_freq,
+                          const OptTensor& positions, double eps, bool interleaved) {
+    CHECK_FLAT16(qkv, qkv, at::kBFloat16);
+    TORCH_CHECK(qkv.dim() == 3 && Hq >= 1 && Hkv >= 1 && qkv.size(2) % (Hq + 2 * Hkv) == 0, "heads: qkv must be [B,T,(Hq + 2 Hkv) D]");
+    const int64_t D = qkv.size(2) / (Hq + 2 * Hkv);
+    TORCH_CHECK(D >= 8 && D % 8 == 0 && D <= 256 && Hq + 2 * Hkv < (1 << 20), "heads: D must be a multiple of 8, <= 256");
+    dpa::HeadsArgs a{};
+    a.qkv = qkv.data_ptr();
+    TORCH_CHECK(qw.has_value() == kw.has_value(), "heads: both gains or none");
+    if (qw.has_value()) {
+        CHECK_FLAT((*qw), qkv, at::kFloat); CHECK_FLAT((*kw), qkv, at::kFloat);
+        TORCH_CHECK(qw->numel() == D && kw->numel() == D, "heads: gains");
+        a.qw = qw->data_ptr<float>(); a.kw = kw->data_ptr<float>();
+    }
+    a.tokens = qkv.size(0) * qkv.size(1);
+    if (inv_freq.has_value()) {
+        CHECK_FLAT((*inv_freq), qkv, at::kDouble);
+        a.R = (int)(2 * inv_freq->numel());
+        TORCH_CHECK(a.R >= 16 && a.R % 16 == 0 && a.R <= D, "heads: rotated channels");
+        a.inv_freq = inv_freq->data_ptr<double>();
+        if (positions.has_value()) {
+            CHECK_FLAT((*positions), qkv, at::kLong);
+            TORCH_CHECK(positions->numel() == a.tokens, "heads: positions");
+            a.positions = positions->data_ptr<int64_t>();
+        }
+    }
+    TORCH_CHECK(qkv.size(1) < (1ll << 31), "heads: oversized problem");
+    a.T = (int)qkv.size(1); a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.D = (int)D; a.interleaved = interleaved; a.eps = (float)eps;
+    return a;
+}
+
+std::vector<Tensor> heads_fwd(const Tensor& qkv, int64_t Hq, int64_t Hkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& inv_freq,
+                              const OptTensor& positions, double eps, bool interleaved) {
+    const dpa::HeadsArgs a = heads_args(qkv, Hq, Hkv, qw, kw, inv_freq, positions, eps, interleaved);
+    Guard guard(qkv.device());
+    Tensor q = torch::empty({qkv.size(0), qkv.size(1), Hq, a.D}, qkv.options()), k = torch::empty({qkv.size(0), qkv.size(1), Hkv, a.D}, qkv.options());
+    if (a.tokens > 0) dpa::heads_fwd(a, q.data_ptr(), k.data_ptr(), cur_stream());
+    return {q, k};
+}
+
+// -> dqkv, dqw, dkw (the last two undefined without gains)
+std::vector<Tensor> heads_bwd(const Tensor& qkv, int64_t Hq, int64_t Hkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& inv_freq,
+                              const OptTensor& positions, double eps, bool interleaved, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
+    const dpa::HeadsArgs a = heads_args(qkv, Hq, Hkv, qw, kw, inv_freq, positions, eps, interleaved);
+    CHECK_FLAT16(dq, qkv, at::kBFloat16); CHECK_FLAT16(dk, qkv, at::kBFloat16); CHECK_FLAT16(dv, qkv, at::kBFloat16);
+    TORCH_CHECK(dq.numel() == a.tokens * Hq * a.D && dk.numel() == a.tokens * Hkv * a.D && dv.numel() == dk.numel(), "heads_bwd: shapes");
+    Guard guard(qkv.device());
+    Tensor dqkv = torch::empty_like(qkv), partial, dw;
+    const auto fopt = qkv.options().dtype(at::kFloat);
+    if (a.qw != nullptr) {
+        if (a.tokens == 0) dw = torch::zeros({2, a.D}, fopt);
+        else { dw = torch::empty({2, a.D}, fopt); partial = torch::empty({2, dpa::heads_partial_rows(a.tokens), a.D}, fopt); }
+    }
+    if (a.tokens > 0)
+        dpa::heads_bwd(a, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dqkv.data_ptr(), a.qw != nullptr ? partial.data_ptr<float>() : nullptr,
+                       a.qw != nullptr ? dw.data_ptr<float>() : nullptr, a.qw != nullptr ? dw.data_ptr<float>() + a.D : nullptr, cur_stream());
+    if (a.qw == nullptr) return {dqkv, Tensor(), Tensor()};
+    return {dqkv, dw[0], dw[1]};
+}
+
+// ---------------------------------------------------------------- token embedding
+bool tok64(const Tensor& tok) {
+    TORCH_CHECK(tok.scalar_type() == at::kLong || tok.scalar_type() == at::kInt, "token_embedding: tokens must be int64 or int32");
+    return tok.scalar_type() == at::kLong;
+}
+
+Tensor token_embedding_fwd(const Tensor& tok, const Tensor& w, double scale) {
+    CHECK_FLAT16(w, w, at::kBFloat16);
+    CHECK_ON(tok, w); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
+    TORCH_CHECK(w.dim() == 2 && w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) < (1 << 24) && w.size(0) >= 1, "token_embedding: table [V, C], C % 8 == 0");
+    const bool t64 = tok64(tok);
+    Guard guard(w.device());
+    auto shape = tok.sizes().vec();
+    shape.push_back(w.size(1));
+    Tensor y = torch::empty(shape, w.options());
+    dpa::token_embedding_fwd(tok.data_ptr(), t64, w.data_ptr(), y.data_ptr(), tok.numel(), (int)w.size(1), w.size(0), (float)scale, cur_stream());
+    return y;
+}
+
+// dw given: the named rows are added to it; else a whole gradient [V, C] is returned
+Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy, int64_t V, double scale, const OptTensor& acc) {
+    CHECK_FLAT16(dy, dy, at::kBFloat16);
+    CHECK_ON(tok, dy); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
+    const int64_t C = dy.size(-1), n = tok.numel();
+    TORCH_CHECK(dy.numel() == n * C && C >= 8 && C % 8 == 0 && C < (1 << 24) && V >= 1 && V < (1ll << 31) - 1 && n < (1ll << 31) - 4096, "token_embedding_bwd: shapes");
+    const bool t64 = tok64(tok), add = acc.has_value();
+    Guard guard(dy.device());
+    const auto fopt = dy.options().dtype(at::kFloat), iopt = dy.options().dtype(at::kInt);
+    Tensor dw;
+    if (add) {
+        dw = *acc;
+        CHECK_FLAT(dw, dy, at::kFloat);
+        TORCH_CHECK(dw.numel() == V * C, "token_embedding_bwd: accumulator");
+    } else {
+        dw = torch::empty({V, C}, fopt);
+    }
+    Tensor scratch = torch::empty({V + 1 + 2 * n}, iopt), partial;
+    const long chunks = dpa::token_embedding_chunks(n);
+    if (chunks > 0) partial = torch::empty({chunks, C}, fopt);
+    int* start = scratch.data_ptr<int>();
+    dpa::token_embedding_bwd(tok.data_ptr(), t64, dy.data_ptr(), dw.data_ptr<float>(), add, n, (int)C, V, (float)scale, start, start + V + 1, start + V + 1 + n,
+                             chunks > 0 ? partial.data_ptr<float>() : nullptr, cur_stream());
+    return dw;
+}
+
+// ---------------------------------------------------------------- distillation
+// -> loss [1], and the logits' gradient for an upstream gradient of 1 (undefined unless asked for)
+std::vector<Tensor> distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool want_grad) {
+    CHECK_ON(logits, logits); TORCH_CHECK(logits.is_contiguous() && logits.dim() == 2, "distill: logits [N, ld], contiguous");
+    const bool bf = logits.scalar_type() == at::kBFloat16;
+    TORCH_CHECK(bf || logits.scalar_type() == at::kFloat, "distill: logits must be bf16 or fp32");
+    CHECK_ON(ids, logits); TORCH_CHECK(ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt), "distill: ids int64 or int32");
+    CHECK_FLAT(teacher, logits, at::kFloat);
+    const int64_t N = logits.size(0), ld = logits.size(1);
+    TORCH_CHECK(ids.dim() == 2 && ids.sizes() == teacher.sizes() && ids.size(0) == N, "distill: ids and teacher [N, K]");
+    const int64_t K = ids.size(1);
+    TORCH_CHECK(K >= 1 && K <= dpa::distill_max_entries() && V >= 1 && V <= ld && ld < (1 << 30) && N < (1ll << 31), "distill: sizes");
+    TORCH_CHECK(tau > 0.0, "distill: temperature");
+    Guard guard(logits.device());
+    const auto fopt = logits.options().dtype(at::kFloat);
+    Tensor loss = torch::empty({1}, fopt), rows = torch::empty({N}, fopt), d;
+    if (want_grad) d = torch::empty_like(logits);
+    dpa::DistillArgs a{};
+    a.logits = logits.data_ptr(); a.dlogits = want_grad ? d.data_ptr() : nullptr;
+    a.ids = ids.data_ptr(); a.teacher = teacher.data_ptr<float>(); a.row_loss = rows.data_ptr<float>();
+    a.N = N; a.ld = ld; a.V = (int)V; a.K = (int)K; a.ids64 = ids.scalar_type() == at::kLong;
+    a.aligned = (ld * (bf ? 2 : 4)) % 16 == 0 && on16(logits) && (!want_grad || on16(d));
+    a.inv_tau = (float)(1.0 / tau);
+    const double n = N > 0 ? (double)N : 1.0;
+    a.grad_scale = (float)(tau / n);
+    dpa::distill(a, bf, (float)(tau * tau / n), loss.data_ptr<float>(), cur_stream());
+    return {loss, d};
+}
+
+void scale_grad(Tensor& d, const Tensor& g) {
+    TORCH_CHECK(d.is_cuda() && d.is_contiguous() && (d.scalar_type() == at::kBFloat16 || d.scalar_type() == at::kFloat), "scale_grad: d");
+    CHECK_FLAT(g, d, at::kFloat);
+    TORCH_CHECK(g.numel() == 1, "scale_grad: g");
+    Guard guard(d.device());
+    if (d.numel() > 0) dpa::scale_grad(d.data_ptr(), d.scalar_type() == at::kBFloat16, g.data_ptr<float>(), d.numel(), cur_stream());
+}
+}  // namespace
+
+void bind_lm(pybind11::module_& m) {
+    m.def("attend_fwd", &attend_fwd);
+    m.def("attend_bwd", &attend_bwd);
+    m.def("heads_fwd", &heads_fwd);
+    m.def("heads_bwd", &heads_bwd);
+    m.def("token_embedding_fwd", &token_embedding_fwd);
+    m.def("token_embedding_bwd", &token_embedding_bwd);
+    m.def("distill", &distill);
+    m.def("scale_grad", &scale_grad);
+}

@@ -241,6 +241,57 @@ void attention_fwd(const void* qkv, void* out, float* lse, int B, int T, int H, 
                    uint64_t offset, hipStream_t st);
 void attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, void* dqkv, float* delta,
                    int B, int T, int H, int D, float drop_p, uint64_t seed, uint64_t offset, hipStream_t st);
+// self-attention with score modifiers (attend.hip): q [B,T,Hq,D], k / v [B,T,Hkv,D] bf16 by element strides (last axis
+// contiguous, every row 16-byte aligned), D % 8 == 0, D <= 128
+struct AttendArgs {
+    const void *q, *k, *v;
+    long qb, qt, qh, kb, kt, kh, vb, vt, vh;
+    const int* docs;                       // [B, T] or nullptr; < 0: padding
+    const int4* ranges;                    // attend_doc_ranges of docs: [B, ceil(T / 64)]
+    const int* prefix;                     // [B] or nullptr
+    const float* slopes;                   // [Hq] or nullptr
+    int B, T, Hq, Hkv, D, causal;
+    float scale, softcap;                  // softcap <= 0: none
+};
+void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t st);
+// lse2 [B, Hq, T]: log2 of the row's sum of 2^score (1e30 for a row that sees nothing)
+void attend_fwd(const AttendArgs& a, void* out, float* lse2, hipStream_t st);
+// out, dout, dq [B,T,Hq,D], dk, dv [B,T,Hkv,D] contiguous; delta [B, Hq, T] is scratch
+void attend_bwd(const AttendArgs& a, const void* out, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st);
+// head norms and rotation over a packed projection [tokens, (Hq + 2 Hkv) * D] bf16 (heads.hip)
+struct HeadsArgs {
+    const void* qkv;
+    const float *qw, *kw;                  // [D] gains, or both nullptr: no norm
+    const double* inv_freq;                // [R / 2]
+    const int64_t* positions;              // [tokens], or nullptr: token % T
+    long tokens;
+    int T, Hq, Hkv, D, R, interleaved;     // D % 8 == 0, D <= 256; R % 16 == 0, R <= D, 0: no rotation
+    float eps;
+};
+void heads_fwd(const HeadsArgs& a, void* q, void* k, hipStream_t st);
+int heads_partial_rows(long tokens);
+// partial [2][heads_partial_rows][D] scratch; dqw / dkw [D] are written (with gains only)
+void heads_bwd(const HeadsArgs& a, const void* dq, const void* dk, const void* dv, void* dqkv, float* partial, float* dqw, float* dkw, hipStream_t st);
+// scaled token embedding and its gradient by sorted tokens (embed.hip); tok int64 (tok64) or int32, C % 8 == 0, n < 2^31
+void token_embedding_fwd(const void* tok, int tok64, const void* w, void* y, long n, int C, long V, float scale, hipStream_t st);
+long token_embedding_chunks(long n);       // rows of `partial`; 0: it may be nullptr
+// start [V + 1], order [n], sorted [n], partial [chunks, C] are scratch; add: into dw, else dw is written whole
+void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, int add, long n, int C, long V, float scale, int* start, int* order,
+                         int* sorted, float* partial, hipStream_t st);
+// distillation from a teacher's top logits (distill.hip)
+struct DistillArgs {
+    const void* logits;                    // [N, ld] bf16 or fp32
+    void* dlogits;                         // same, or nullptr: no gradient
+    const void* ids;                       // [N, K] int64 (ids64) or int32
+    const float* teacher;                  // [N, K]
+    float* row_loss;                       // [N] scratch
+    long N, ld;
+    int V, K, ids64, aligned;              // aligned: every row of both tensors on 16 bytes
+    float inv_tau, grad_scale;             // 1 / tau, tau / N
+};
+int distill_max_entries();
+void distill(const DistillArgs& a, int is_bf16, float loss_scale /* tau^2 / N */, float* loss, hipStream_t st);
+void scale_grad(void* d, int is_bf16, const float* g, long n, hipStream_t st);   // d *= *g unless *g is 1
 // y = addend + x * keep(seed, offset, i) / (1 - p)  (bf16, n % 8 == 0; addend optional): element dropout with the mask
 // drawn in line, fused with the residual add that follows it in a transformer block
 void dropout_bf16(const void* x, const void* addend, void* y, long n, float p, uint64_t seed, uint64_t offset, hipStream_t st);

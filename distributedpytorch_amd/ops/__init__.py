@@ -12,3 +12,7 @@ from .misc import (max_pool_3x3_s2_nhwc, global_avg_pool_nhwc, to_nhwc, add_relu
 from .loss import softmax_cross_entropy  # noqa: F401
 from .small import (conv5_pool_relu, linear_f32, linear_log_softmax, linear_log_softmax_nll, dropout, channel_dropout_mask, log_softmax, nll_loss)  # noqa: F401
 from .tfm import embedding, causal_attention, dropout_residual  # noqa: F401
+from .attend import attention  # noqa: F401
+from .heads import qk_norm_rotary, rotary_frequencies  # noqa: F401
+from .embed import token_embedding  # noqa: F401
+from .distill import distillation_loss  # noqa: F401
