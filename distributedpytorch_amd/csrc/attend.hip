@@ -14,7 +14,10 @@
 //   * Scores are kept in the exponent's base 2 throughout; tanh(x) = 1 - 2 r with r = 1 / (1 + e^{2x}), so that
 //     1 - tanh^2 = 4 r (1 - r) costs no second transcendental in the backward kernels.
 //   * delta comes from the same MFMA as dP (the diagonal of O dO^T): a row with one visible key has dP = delta bit for
-//     bit, and its dS is exactly zero as the formula says.
+//     bit, and its dS is exactly zero as the formula says.  O enters it with what its rounding took away (kept by the
+//     forward in bf16, `rest`): where a few keys carry a row, dS is a small difference of dP and delta, and delta from the
+//     rounded O alone costs dQ and dK as much accuracy as their own rounding does (3.8e-3 against 2.5e-3 of the norm at
+//     scores of standard deviation 8 under a cap of 30).
 //   * Rows behind a document number < 0 are staged as zeros: whatever a padded row holds reaches no product.
 #include <math.h>
 #include "attn_tile.h"
@@ -169,7 +172,7 @@ __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& r)
 
 // ------------------------------------------------------------------------------ forward
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(AttendArgs a, unsigned short* __restrict__ out, float* __restrict__ lse2) {
+__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(AttendArgs a, unsigned short* __restrict__ out, unsigned short* __restrict__ rest, float* __restrict__ lse2) {
     constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>();
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * TB + TILE * 4];
     unsigned char* Ks = smem;
@@ -292,14 +295,29 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(Atten
     }
     if (q < T) {
         const bool empty = l == 0.f;                                // saw no key: output zero, and P = exp2(x - 1e30) = 0 in backward
-        store_cols<DH>(out + (((long)b * T + q) * a.Hq + head) * a.D, O, empty ? 0.f : 1.f / l, h, a.D);
+        // a sum this near 1 is one key's exponent off by its own rounding: taken as 1, so that O is that key's V exactly
+        const bool one = fabsf(l - 1.f) <= 2.384185791015625e-7f * fmaxf(1.f, fabsf(m));
+        const float inv = empty ? 0.f : one ? 1.f : 1.f / l;
+        const long row = (((long)b * T + q) * a.Hq + head) * a.D;
+#pragma unroll
+        for (int di = 0; di < DI; ++di)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[di][r] *= inv;
+        store_cols<DH>(out + row, O, 1.f, h, a.D);
+        if (rest != nullptr) {
+#pragma unroll
+            for (int di = 0; di < DI; ++di)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) O[di][r] -= bf16_to_float(float_to_bf16(O[di][r]));
+            store_cols<DH>(rest + row, O, 1.f, h, a.D);
+        }
         if (h == 0) lse2[((long)b * a.Hq + head) * T + q] = empty ? 1.0e30f : m + __log2f(l);
     }
 }
 
 // ------------------------------------------------------------------------------ dQ (query-stationary), and delta
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(AttendArgs a, const unsigned short* __restrict__ out,
+__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(AttendArgs a, const unsigned short* __restrict__ out, const unsigned short* __restrict__ rest,
                                                                             const unsigned short* __restrict__ dout, const float* __restrict__ lse2,
                                                                             float* __restrict__ delta, unsigned short* __restrict__ dq) {
     constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>();
@@ -332,6 +350,9 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(Att
         load_frags<DH>(out + orow, h, a.D, qdoc >= 0, of);
         floatx16 dd;
         zero16(dd);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) dd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(of[kk], dof[kk], dd, 0, 0, 0);
+        load_frags<DH>(rest + orow, h, a.D, qdoc >= 0, of);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) dd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(of[kk], dof[kk], dd, 0, 0, 0);
         del = 0.f;
@@ -548,14 +569,15 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_kv_kernel(At
 }
 
 template <int DH, bool CAP, bool BIAS>
-void fwd_of(const AttendArgs& a, void* out, float* lse2, hipStream_t st) {
-    hipLaunchKernelGGL((attend_fwd_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, (a.T + BQ - 1) / BQ), dim3(256), 0, st, a, (unsigned short*)out, lse2);
+void fwd_of(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) {
+    hipLaunchKernelGGL((attend_fwd_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, (a.T + BQ - 1) / BQ), dim3(256), 0, st, a, (unsigned short*)out,
+                       (unsigned short*)rest, lse2);
 }
 template <int DH, bool CAP, bool BIAS>
-void bwd_of(const AttendArgs& a, const void* out, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
+void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
     const int blocks = (a.T + BQ - 1) / BQ;
     hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
-                       (const unsigned short*)dout, lse2, delta, (unsigned short*)dq);
+                       (const unsigned short*)rest, (const unsigned short*)dout, lse2, delta, (unsigned short*)dq);
     hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout,
                        lse2, delta, (unsigned short*)dk, (unsigned short*)dv);
 }
@@ -580,10 +602,10 @@ void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t 
     hipLaunchKernelGGL(doc_ranges_kernel, dim3((tiles + 3) / 4, B), dim3(256), 0, st, docs, (int4*)ranges, T, tiles);
 }
 
-void attend_fwd(const AttendArgs& a, void* out, float* lse2, hipStream_t st) { DPA_ATTEND_PICK(fwd_of, a, out, lse2, st); }
+void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) { DPA_ATTEND_PICK(fwd_of, a, out, rest, lse2, st); }
 
-void attend_bwd(const AttendArgs& a, const void* out, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
-    DPA_ATTEND_PICK(bwd_of, a, out, dout, lse2, delta, dq, dk, dv, st);
+void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
+    DPA_ATTEND_PICK(bwd_of, a, out, rest, dout, lse2, delta, dq, dk, dv, st);
 }
 
 }  // namespace dpa

@@ -1,6 +1,9 @@
 // Bindings for the language-model kernels: attention with score modifiers, head norms with rotation, the scaled token
-// embedding and the distillation loss.  The Python side (ops/attend.py, ops/heads.py, ops/embed.py, ops/distill.py) states
-// what a call may be; the checks here are what the kernels' addressing relies on.
+// embedding and the distillation loss, each as an autograd node of its own.  The Python side (ops/attend.py, ops/heads.py,
+// ops/embed.py, ops/distill.py) states what a call may be; the checks here are what the kernels' addressing relies on.
+//
+// The nodes are C++ and not Python functions because the smallest calls are all host time: the engine runs a backward on a
+// thread of its own, and a Python node has to win the interpreter lock there first.
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -18,6 +21,23 @@ using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
                                        TORCH_CHECK((t).scalar_type() == (type), #t ": wrong type"); } while (0)
 inline bool on16(const Tensor& t) { return ((uintptr_t)t.data_ptr()) % 16 == 0; }
 #define CHECK_FLAT16(t, like, type) do { CHECK_FLAT(t, like, type); TORCH_CHECK(on16(t), #t " must be 16-byte aligned"); } while (0)
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The kernels form first derivatives only.
+void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "this operator's gradient cannot be differentiated again"); }
+
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor bare(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+Tensor flat16(const Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// last axis contiguous, every row on 16 bytes
+Tensor rows16(const Tensor& t) {
+    bool ok = on16(t) && (t.size(-1) <= 1 || t.stride(-1) == 1);
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 // ---------------------------------------------------------------- attention
 // element stride of axis i (0 where the axis has one entry), in whole 16-byte steps
@@ -64,31 +84,32 @@ dpa::AttendArgs attend_args(const Tensor& q, const Tensor& k, const Tensor& v, b
     return a;
 }
 
-// -> out [B,T,Hq,D], lse2 [B,Hq,T], ranges (undefined without documents)
+// -> out [B,T,Hq,D], lse2 [B,Hq,T], ranges (undefined without documents), rest (what rounding took from out; for backward)
 std::vector<Tensor> attend_fwd(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
-                               const OptTensor& documents, const OptTensor& prefix) {
+                               const OptTensor& documents, const OptTensor& prefix, bool for_backward) {
     dpa::AttendArgs a = attend_args(q, k, v, causal, scale, softcap, slopes, documents, prefix);
     Guard guard(q.device());
-    Tensor out = torch::empty(q.sizes(), q.options());
+    Tensor out = torch::empty(q.sizes(), q.options()), rest;
     Tensor lse2 = torch::empty({a.B, a.Hq, a.T}, q.options().dtype(at::kFloat));
     Tensor ranges;
-    if (out.numel() == 0) return {out, lse2, ranges};
+    if (for_backward) rest = torch::empty(q.sizes(), q.options());
+    if (out.numel() == 0) return {out, lse2, ranges, rest};
     if (a.docs != nullptr) {
         ranges = torch::empty({a.B, (a.T + 63) / 64, 4}, q.options().dtype(at::kInt));
         dpa::attend_doc_ranges(a.docs, ranges.data_ptr(), a.B, a.T, cur_stream());
         a.ranges = (const int4*)ranges.data_ptr();
     }
-    dpa::attend_fwd(a, out.data_ptr(), lse2.data_ptr<float>(), cur_stream());
-    return {out, lse2, ranges};
+    dpa::attend_fwd(a, out.data_ptr(), for_backward ? rest.data_ptr() : nullptr, lse2.data_ptr<float>(), cur_stream());
+    return {out, lse2, ranges, rest};
 }
 
 // -> dq, dk, dv, contiguous
 std::vector<Tensor> attend_bwd(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
-                               const OptTensor& documents, const OptTensor& prefix, const OptTensor& ranges, const Tensor& out, const Tensor& dout,
-                               const Tensor& lse2) {
+                               const OptTensor& documents, const OptTensor& prefix, const OptTensor& ranges, const Tensor& out, const Tensor& rest,
+                               const Tensor& dout, const Tensor& lse2) {
     dpa::AttendArgs a = attend_args(q, k, v, causal, scale, softcap, slopes, documents, prefix);
-    CHECK_FLAT16(out, q, at::kBFloat16); CHECK_FLAT16(dout, q, at::kBFloat16); CHECK_FLAT(lse2, q, at::kFloat);
-    TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes() && lse2.numel() == (int64_t)a.B * a.Hq * a.T, "attend_bwd: shapes");
+    CHECK_FLAT16(out, q, at::kBFloat16); CHECK_FLAT16(rest, q, at::kBFloat16); CHECK_FLAT16(dout, q, at::kBFloat16); CHECK_FLAT(lse2, q, at::kFloat);
+    TORCH_CHECK(out.sizes() == q.sizes() && rest.sizes() == q.sizes() && dout.sizes() == q.sizes() && lse2.numel() == (int64_t)a.B * a.Hq * a.T, "attend_bwd: shapes");
     Guard guard(q.device());
     Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), q.options()), dv = torch::empty(k.sizes(), q.options());
     if (out.numel() == 0) return {dq, dk, dv};
@@ -98,9 +119,34 @@ std::vector<Tensor> attend_bwd(const Tensor& q, const Tensor& k, const Tensor& v
         a.ranges = (const int4*)ranges->data_ptr();
     }
     Tensor delta = torch::empty_like(lse2);
-    dpa::attend_bwd(a, out.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    dpa::attend_bwd(a, out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                     cur_stream());
     return {dq, dk, dv};
+}
+
+struct AttendNode : public torch::autograd::Function<AttendNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, bool causal, double scale, double softcap,
+                          const OptTensor& slopes, const OptTensor& documents, const OptTensor& prefix, bool for_backward) {
+        const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
+        auto r = attend_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix, for_backward);
+        if (for_backward) {
+            ctx->save_for_backward({q, k, v, bare(slopes), bare(documents), bare(prefix), r[2], r[0], r[3], r[1]});
+            ctx->saved_data["causal"] = causal; ctx->saved_data["scale"] = scale; ctx->saved_data["softcap"] = softcap;
+        }
+        return r[0];
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once();
+        const auto s = ctx->get_saved_variables();
+        auto d = attend_bwd(s[0], s[1], s[2], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(),
+                            opt(s[3]), opt(s[4]), opt(s[5]), opt(s[6]), s[7], s[8], flat16(g[0]), s[9]);
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+Tensor attention_ex(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale, double softcap, const OptTensor& slopes,
+                    const OptTensor& documents, const OptTensor& prefix) {
+    const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    return AttendNode::apply(q, k, v, causal, scale, softcap, slopes, documents, prefix, grad);
 }
 
 // ---------------------------------------------------------------- head norms and rotation
@@ -164,13 +210,40 @@ std::vector<Tensor> heads_bwd(const Tensor& qkv, int64_t Hq, int64_t Hkv, const 
     return {dqkv, dw[0], dw[1]};
 }
 
+struct HeadsNode : public torch::autograd::Function<HeadsNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& inv_freq,
+                                 const OptTensor& positions, int64_t Hq, int64_t Hkv, double eps, bool interleaved) {
+        const Tensor x = flat16(qkv);
+        auto r = heads_fwd(x, Hq, Hkv, qw, kw, inv_freq, positions, eps, interleaved);
+        ctx->save_for_backward({x, bare(qw), bare(kw), bare(inv_freq), bare(positions)});
+        ctx->saved_data["Hq"] = Hq; ctx->saved_data["Hkv"] = Hkv; ctx->saved_data["eps"] = eps; ctx->saved_data["interleaved"] = interleaved;
+        const int64_t n = Hq + 2 * Hkv;
+        return {r[0], r[1], qkv.view({qkv.size(0), qkv.size(1), n, qkv.size(2) / n}).narrow(2, Hq + Hkv, Hkv)};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once();
+        const auto s = ctx->get_saved_variables();
+        const int64_t Hq = ctx->saved_data["Hq"].toInt(), Hkv = ctx->saved_data["Hkv"].toInt(), D = s[0].size(2) / (Hq + 2 * Hkv);
+        // an output that nothing used has no gradient
+        auto given = [&](const Tensor& t, int64_t h) { return t.defined() ? flat16(t) : torch::zeros({s[0].size(0), s[0].size(1), h, D}, s[0].options()); };
+        auto d = heads_bwd(s[0], Hq, Hkv, opt(s[1]), opt(s[2]), opt(s[3]), opt(s[4]), ctx->saved_data["eps"].toDouble(),
+                           ctx->saved_data["interleaved"].toBool(), given(g[0], Hq), given(g[1], Hkv), given(g[2], Hkv));
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+variable_list qk_norm_rotary(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& inv_freq, const OptTensor& positions, int64_t Hq,
+                             int64_t Hkv, double eps, bool interleaved) {
+    return HeadsNode::apply(qkv, qw, kw, inv_freq, positions, Hq, Hkv, eps, interleaved);
+}
+
 // ---------------------------------------------------------------- token embedding
 bool tok64(const Tensor& tok) {
     TORCH_CHECK(tok.scalar_type() == at::kLong || tok.scalar_type() == at::kInt, "token_embedding: tokens must be int64 or int32");
     return tok.scalar_type() == at::kLong;
 }
 
-Tensor token_embedding_fwd(const Tensor& tok, const Tensor& w, double scale) {
+Tensor token_embedding_fwd(const Tensor& tok, const Tensor& w_, double scale) {
+    const Tensor w = flat16(w_);
     CHECK_FLAT16(w, w, at::kBFloat16);
     CHECK_ON(tok, w); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
     TORCH_CHECK(w.dim() == 2 && w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) < (1 << 24) && w.size(0) >= 1, "token_embedding: table [V, C], C % 8 == 0");
@@ -184,7 +257,8 @@ Tensor token_embedding_fwd(const Tensor& tok, const Tensor& w, double scale) {
 }
 
 // dw given: the named rows are added to it; else a whole gradient [V, C] is returned
-Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy, int64_t V, double scale, const OptTensor& acc) {
+Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy_, int64_t V, double scale, const OptTensor& acc) {
+    const Tensor dy = flat16(dy_);
     CHECK_FLAT16(dy, dy, at::kBFloat16);
     CHECK_ON(tok, dy); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
     const int64_t C = dy.size(-1), n = tok.numel();
@@ -208,6 +282,20 @@ Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy, int64_t V, doubl
                              chunks > 0 ? partial.data_ptr<float>() : nullptr, cur_stream());
     return dw;
 }
+
+struct EmbedNode : public torch::autograd::Function<EmbedNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& tok, const Tensor& w, const Tensor& w_lp, double scale) {
+        ctx->save_for_backward({tok});
+        ctx->saved_data["scale"] = scale; ctx->saved_data["V"] = w.size(0);
+        return token_embedding_fwd(tok, w_lp, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once();
+        const auto s = ctx->get_saved_variables();
+        return {Tensor(), token_embedding_bwd(s[0], g[0], ctx->saved_data["V"].toInt(), ctx->saved_data["scale"].toDouble(), c10::nullopt), Tensor(), Tensor()};
+    }
+};
+Tensor token_embedding(const Tensor& tok, const Tensor& w, const Tensor& w_lp, double scale) { return EmbedNode::apply(tok, w, w_lp, scale); }
 
 // ---------------------------------------------------------------- distillation
 // -> loss [1], and the logits' gradient for an upstream gradient of 1 (undefined unless asked for)
@@ -245,15 +333,42 @@ void scale_grad(Tensor& d, const Tensor& g) {
     Guard guard(d.device());
     if (d.numel() > 0) dpa::scale_grad(d.data_ptr(), d.scalar_type() == at::kBFloat16, g.data_ptr<float>(), d.numel(), cur_stream());
 }
+// When a gradient will be asked for the forward kernel writes it beside the loss, for an upstream gradient of 1; backward
+// multiplies by the real one only when it is not 1 (tested on the device).  A second backward through the node forms it again.
+struct DistillNode : public torch::autograd::Function<DistillNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool for_backward) {
+        auto r = distill(logits, ids, teacher, V, tau, for_backward);
+        if (for_backward) {
+            ctx->save_for_backward({logits, ids, teacher});
+            ctx->saved_data["V"] = V; ctx->saved_data["tau"] = tau; ctx->saved_data["d"] = r[1];
+        }
+        return r[0].view(at::IntArrayRef());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once();
+        const auto s = ctx->get_saved_variables();
+        Tensor d;
+        const auto at = ctx->saved_data.find("d");
+        if (at != ctx->saved_data.end()) {
+            d = at->second.toTensor();
+            ctx->saved_data.erase(at);
+        } else {
+            d = distill(s[0], s[1], s[2], ctx->saved_data["V"].toInt(), ctx->saved_data["tau"].toDouble(), true)[1];
+        }
+        scale_grad(d, g[0].reshape({1}));
+        return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+Tensor distillation_loss(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau) {
+    return DistillNode::apply(logits, ids, teacher, V, tau, at::GradMode::is_enabled() && logits.requires_grad());
+}
 }  // namespace
 
 void bind_lm(pybind11::module_& m) {
-    m.def("attend_fwd", &attend_fwd);
-    m.def("attend_bwd", &attend_bwd);
-    m.def("heads_fwd", &heads_fwd);
-    m.def("heads_bwd", &heads_bwd);
+    m.def("attention_ex", &attention_ex);
+    m.def("qk_norm_rotary", &qk_norm_rotary);
+    m.def("token_embedding", &token_embedding);
     m.def("token_embedding_fwd", &token_embedding_fwd);
     m.def("token_embedding_bwd", &token_embedding_bwd);
-    m.def("distill", &distill);
-    m.def("scale_grad", &scale_grad);
+    m.def("distillation_loss", &distillation_loss);
 }

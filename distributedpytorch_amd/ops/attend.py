@@ -10,41 +10,8 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels read it: last axis contiguous, every row on 16 bytes; copied only where it is not so already."""
-    if (t.stride(-1) == 1 or t.size(-1) == 1) and all(s % 8 == 0 or n <= 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])) \
-            and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _flat16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and on 16 bytes."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-class _AttendFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, causal, scale, softcap, slopes, documents, prefix):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out, lse2, ranges = _ext.load().attend_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)
-        ctx.save_for_backward(q, k, v, slopes, documents, prefix, ranges, out, lse2)
-        ctx.meta = (causal, scale, softcap)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, slopes, documents, prefix, ranges, out, lse2 = ctx.saved_tensors
-        dq, dk, dv = _ext.load().attend_bwd(q, k, v, *ctx.meta, slopes, documents, prefix, ranges, out, _flat16(dout), lse2)
-        return dq, dk, dv, None, None, None, None, None, None
 
 
 def _visible(B, T, causal, documents, prefix, device):
@@ -135,4 +102,4 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     if B > 65535 or Hq > 65535 or T > 1 << 22:
         raise ValueError("attention: at most 65,535 rows, 65,535 heads and 4,194,304 tokens in a row")
     slopes, documents, prefix = (t if t is None else t.contiguous() for t in (slopes, documents, prefix))
-    return _AttendFn.apply(q, k, v, bool(causal), scale, softcap, slopes, documents, prefix)
+    return _ext.load().attention_ex(q, k, v, bool(causal), scale, softcap, slopes, documents, prefix)

@@ -8,35 +8,10 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 
 MAX_ENTRIES = 1024                       # teacher entries of a row on the GPU: one per thread of a workgroup
-
-
-class _DistillFn(torch.autograd.Function):
-    """When a gradient will be asked for the forward kernel writes it beside the loss (for an upstream gradient of 1);
-    backward multiplies by the real upstream gradient only when it is not 1 (tested on the device).  A second backward
-    through the same node forms the gradient again."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, n_classes, temperature):
-        loss, ctx.d = _ext.load().distill(logits, ids, teacher, n_classes, temperature, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, ids, teacher)
-        ctx.meta = (n_classes, temperature)
-        return loss.view(())
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, ids, teacher = ctx.saved_tensors
-        C = _ext.load()
-        d, ctx.d = ctx.d, None
-        if d is None:
-            d = C.distill(logits, ids, teacher, *ctx.meta, True)[1]
-        C.scale_grad(d, g.reshape(1))
-        return d, None, None, None, None
 
 
 def _plain(logits, ids, teacher, n_classes, tau):
@@ -99,4 +74,4 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         raise ValueError(f"distillation_loss: {K} teacher entries per row, at most {MAX_ENTRIES} on the GPU")
     if ld >= 1 << 30 or logits.shape[0] >= 1 << 31:
         raise ValueError("distillation_loss: at most 2^30 - 1 columns and 2^31 - 1 rows")
-    return _DistillFn.apply(logits.contiguous(), teacher_ids.contiguous(), teacher_logits.contiguous(), n_classes, temperature)
+    return _ext.load().distillation_loss(logits.contiguous(), teacher_ids.contiguous(), teacher_logits.contiguous(), n_classes, temperature)

@@ -11,10 +11,11 @@ from torch.autograd.function import once_differentiable
 
 from . import _ext
 from . import sink as _sink
-from .attend import _flat16
 
 
-class _TokenEmbeddingFn(torch.autograd.Function):
+class _SinkEmbeddingFn(torch.autograd.Function):
+    """The node for a weight with a gradient sink: backward adds into the sink's buffer and reports the parameter."""
+
     @staticmethod
     def forward(ctx, tokens, weight, weight_lp, scale):
         ctx.save_for_backward(tokens)
@@ -27,7 +28,7 @@ class _TokenEmbeddingFn(torch.autograd.Function):
         (tokens,) = ctx.saved_tensors
         weight = ctx.weight
         acc = _sink.target(weight)
-        dw = _ext.load().token_embedding_bwd(tokens, _flat16(dy), weight.shape[0], ctx.scale, None if acc is None else acc.view(weight.shape))
+        dw = _ext.load().token_embedding_bwd(tokens, dy, weight.shape[0], ctx.scale, None if acc is None else acc.view(weight.shape))
         if acc is not None:
             _sink.ready(weight)
             dw = None
@@ -63,4 +64,5 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, weight_lp: torch
         weight_lp = _lp(weight, None)
     elif weight_lp.shape != weight.shape or weight_lp.dtype != torch.bfloat16 or weight_lp.device != weight.device:
         raise ValueError("token_embedding: weight_lp must be the bf16 shadow of weight")
-    return _TokenEmbeddingFn.apply(tokens.contiguous(), weight, _flat16(weight_lp), scale)
+    node = _ext.load().token_embedding if _sink.of(weight) is None else _SinkEmbeddingFn.apply
+    return node(tokens.contiguous(), weight, weight_lp, scale)

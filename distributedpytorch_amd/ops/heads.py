@@ -7,10 +7,8 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
-from .attend import _flat16
 
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -18,26 +16,6 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, device=None) -> 
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_frequencies: rotary_dim must be even and positive, got {rotary_dim}")
     return float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
-
-
-class _HeadsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, q_weight, k_weight, inv_freq, positions, n_head, n_kv_head, eps, interleaved):
-        x = _flat16(qkv)
-        q, k = _ext.load().heads_fwd(x, n_head, n_kv_head, q_weight, k_weight, inv_freq, positions, eps, interleaved)
-        ctx.save_for_backward(x, q_weight, k_weight, inv_freq, positions)
-        ctx.meta = (n_head, n_kv_head, eps, interleaved)
-        v = qkv.view(*q.shape[:2], n_head + 2 * n_kv_head, q.shape[3])[:, :, n_head + n_kv_head:]
-        return q, k, v
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk, dv):
-        x, q_weight, k_weight, inv_freq, positions = ctx.saved_tensors
-        n_head, n_kv_head, eps, interleaved = ctx.meta
-        dqkv, dqw, dkw = _ext.load().heads_bwd(x, n_head, n_kv_head, q_weight, k_weight, inv_freq, positions, eps, interleaved,
-                                               _flat16(dq), _flat16(dk), _flat16(dv))
-        return dqkv, dqw, dkw, None, None, None, None, None, None
 
 
 def _plain(qkv, n_head, n_kv_head, q_weight, k_weight, inv_freq, positions, eps, interleaved):
@@ -118,4 +96,4 @@ def qk_norm_rotary(qkv: torch.Tensor, n_head: int, n_kv_head: Optional[int] = No
     if not qkv.is_contiguous():
         qkv = qkv.contiguous()
     q_weight, k_weight, inv_freq, positions = (t if t is None else t.contiguous() for t in (q_weight, k_weight, inv_freq, positions))
-    return _HeadsFn.apply(qkv, q_weight, k_weight, inv_freq, positions, n_head, n_kv_head, float(eps), bool(interleaved))
+    return tuple(_ext.load().qk_norm_rotary(qkv, q_weight, k_weight, inv_freq, positions, n_head, n_kv_head, float(eps), bool(interleaved)))

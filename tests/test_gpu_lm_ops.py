@@ -533,6 +533,17 @@ def test_pass_on_another_stream_and_in_replayed_graphs(which):
                 t.fill_(7)                          # a replay has to write everything again
 
 
+@pytest.mark.parametrize("which", ["attend", "heads", "embed", "distil"])
+def test_no_second_derivative(which):
+    x = {"attend": lambda: _rand(1, 5, 2, 64), "heads": lambda: _rand(1, 5, 192), "embed": lambda: _rand(9, 8, dtype=torch.float32),
+         "distil": lambda: _rand(3, 20)}[which]().to(DEV).requires_grad_()
+    y = {"attend": lambda: ops.attention(x, x, x), "heads": lambda: ops.qk_norm_rotary(x, 1, inv_freq=ops.rotary_frequencies(64, device=DEV))[0],
+         "embed": lambda: ops.token_embedding(torch.tensor([1, 2], device=DEV), x),
+         "distil": lambda: ops.distillation_loss(x, torch.tensor([[1], [2], [3]], device=DEV), torch.zeros(3, 1, device=DEV))}[which]()
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
 def test_gpu_refusals():
     b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
     for bad in ((b(1, 4, 2, 136),) * 3, (b(1, 4, 2, 12),) * 3):
