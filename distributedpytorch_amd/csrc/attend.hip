@@ -73,12 +73,12 @@ struct TileWalk {
     const int4* rg;                      // nullptr: no documents, every tile is visited whole
     int base, end, j;
     DocRange block, wave;
-    unsigned long long todo, mine_bits, whole_bits;
-    bool mine, whole;
+    unsigned long long todo, mine_bits, whole_bits, pad_bits;
+    bool mine, whole, pad;                // pad: some of the tile's rows are padding
 
     __device__ __forceinline__ void look() {
         const int lane = threadIdx.x & 63, t = base + lane;
-        bool a = t < end, b = true, c = true;
+        bool a = t < end, b = true, c = true, p = false;
         if (rg != nullptr) {
             DocRange d{0x7fffffff, -0x7fffffff};
             if (a) {
@@ -88,8 +88,9 @@ struct TileWalk {
             a = a && meets(d, block);
             b = meets(d, wave);
             c = same_doc(d, wave);
+            p = d.lo < 0;
         }
-        todo = __ballot(a); mine_bits = __ballot(b); whole_bits = __ballot(c);
+        todo = __ballot(a); mine_bits = __ballot(b); whole_bits = __ballot(c); pad_bits = __ballot(p);
     }
     __device__ __forceinline__ void start(int first, int end_) { base = first; end = end_; look(); }
     // the next tile, or `end` when there is none
@@ -101,33 +102,90 @@ struct TileWalk {
         }
         const int bit = __ffsll((long long)todo) - 1;
         todo &= todo - 1;
-        mine = (mine_bits >> bit) & 1; whole = (whole_bits >> bit) & 1;
+        mine = (mine_bits >> bit) & 1; whole = (whole_bits >> bit) & 1; pad = (pad_bits >> bit) & 1;
         return base + bit;
     }
 };
 
-// A 64 x DH tile on its way to LDS.  Rows past T and rows of padding become zeros; columns past D repeat the last eight (the
-// other operand of every product that sums over them is zero there).
+// 64 rows x DH columns from memory straight into an LDS image (img_off), 16 bytes a lane and no registers in between: a wave's
+// instruction fills 1 KiB in lane order, so the image's swizzle goes into which 16 bytes of the row each lane asks for.
+// Rows past the last one are past the end of the descriptor and arrive as zeros; columns past D repeat the last eight (the
+// other operand of every product that sums over them is zero there).  Completion: tiles_landed(), then a barrier.
 template <int DH>
-struct Staged {
-    u32x4 r[DH / 32];
-    int doc[DH / 32];
-    __device__ __forceinline__ void fetch(const unsigned short* __restrict__ g, long rs, int r0, int T, int D, const int* __restrict__ docs, int tid) {
-        constexpr int CPR = DH / 8, RSTEP = 256 / CPR;
-        const int col = min((tid % CPR) * 8, D - 8);
-#pragma unroll
-        for (int i = 0; i < DH / 32; ++i) {
-            const int row = r0 + tid / CPR + i * RSTEP, rc = min(row, T - 1);
-            r[i] = *(const u32x4*)(g + (long)rc * rs + col);
-            doc[i] = row < T ? (docs != nullptr ? docs[rc] : 0) : -1;
-        }
+struct TileDma {
+    const unsigned short* base;          // row 0
+    long rs;                             // row stride, elements
+    unsigned off;                        // this lane's bytes in the tile's first rows
+    int T, D;
+    __device__ __forceinline__ TileDma(const unsigned short* g, long rs_, int T_, int D_, int tid) : base(g), rs(rs_), T(T_), D(D_) {
+        constexpr int CPR = DH / 8;
+        const int row = tid / CPR, slot = tid % CPR;
+        const int key = DH == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
+        off = (unsigned)(row * rs * 2) + 2 * min((slot ^ key) * 8, D - 8);
     }
-    __device__ __forceinline__ void stash(unsigned char* lds, int tid) const {
-        constexpr int CPR = DH / 8, RSTEP = 256 / CPR;
-        const int c = tid % CPR;
+    __device__ __forceinline__ void fetch(unsigned char* lds, int r0, int wave) const {
+        constexpr int RSTEP = 256 / (DH / 8);                        // rows a workgroup's instruction covers: a multiple of 16, so `key` repeats
+        const u32x4 words = buffer_words(base + (long)r0 * rs, (unsigned)(((min(TILE, T - r0) - 1) * rs + D) * 2));
+        unsigned o = off;
+        asm volatile("" : "+v"(o));                                  // the sums below are formed here, not kept across the loop
 #pragma unroll
         for (int i = 0; i < DH / 32; ++i)
-            *(u32x4*)(lds + img_off<DH>(tid / CPR + i * RSTEP, c * 8)) = doc[i] < 0 ? u32x4{0, 0, 0, 0} : r[i];
+            dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + (unsigned)(i * RSTEP * rs * 2));
+    }
+};
+// 64 words (documents, statistics) into LDS by one wave, a word a lane; zeros from word `n` on
+__device__ __forceinline__ void fetch_words(void* lds, const void* from, long n, int lane) {
+    typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
+    const unsigned at = (unsigned)(unsigned long long)(lds_byte_ptr)(unsigned char*)lds;
+    const u32x4 words = buffer_words(from, (unsigned)(min(n, 64L) * 4));
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(words), "s"(at) : "memory");
+}
+// every load that this wave has issued is done
+__device__ __forceinline__ void tiles_landed() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// rows of padding become zeros (docs: the tile's 64 document numbers in LDS)
+template <int DH>
+__device__ __forceinline__ void clear_padding(unsigned char* lds, const int* docs, int tid) {
+    constexpr int CPR = DH / 8, RSTEP = 256 / CPR;
+    u32x4 zero = {0, 0, 0, 0};
+    asm volatile("" : "+v"(zero));                                   // formed here, not kept across the loop
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) {
+        const int row = tid / CPR + i * RSTEP;
+        if (docs[row] < 0) *(u32x4*)(lds + row * DH * 2 + (tid % CPR) * 16) = zero;
+    }
+}
+
+// Where a lane reads its fragments in an image (img_off): the swizzle is an XOR of bits that lie below a row's size, so one
+// offset per kind of read and an XOR with a constant give every fragment's place - 16 offsets kept in registers instead
+// put the backward kernels past their budget.
+template <int DH>
+struct FragAt {
+    int row, tr;
+    __device__ __forceinline__ explicit FragAt(int lane) {
+        const int r = lane & 31, h = lane >> 5, tq = (lane & 15) >> 2, tp = lane & 3, gi = (lane >> 4) & 1;
+        row = img_off<DH>(r, 8 * h);
+        tr = img_off<DH>(4 * h + tq, 16 * gi + 4 * tp);
+    }
+    // a copy whose offsets the compiler takes for new ones: it forms the XORs where they are used instead of keeping all of
+    // them in registers across the loop
+    __device__ __forceinline__ FragAt fresh() const {
+        FragAt f = *this;
+        asm volatile("" : "+v"(f.row), "+v"(f.tr));
+        return f;
+    }
+    // A / B fragment kk of row 32 t2 + (lane & 31): elements 16 kk + 8 h ..
+    __device__ __forceinline__ bf16x8 rows(const unsigned char* img, int t2, int kk) const {
+        return *(const bf16x8*)(img + (row ^ (kk << 5)) + 32 * t2 * DH * 2);
+    }
+    // transposed A fragment (tr_frag) of rows 32 t2 + 16 s + 4 h .., columns 32 di + (lane & 31)
+    __device__ __forceinline__ bf16x8 cols(const unsigned char* img, int t2, int s, int di) const {
+        const unsigned char* at = img + (32 * t2 + 16 * s) * DH * 2;
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(at + (tr ^ (di << 6))));
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(at + (tr ^ (di << 6) ^ 32) + 8 * DH * 2));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
 
@@ -159,8 +217,11 @@ __device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, con
         }
 }
 
-// score of a pair in base 2 from the raw product; `r` (cap only): 1 / (1 + e^{2x}), from which 1 - tanh^2 = 4 r (1 - r)
+// Scores in base 2 from raw products.  `r` (cap only): 1 / (1 + e^{2x}), from which 1 - tanh^2 = 4 r (1 - r).
 struct ScoreMap { float c, k1, cap2; };       // scale log2 e;  2 scale log2 e / cap;  cap log2 e
+__device__ __forceinline__ ScoreMap score_map(const AttendArgs& a, bool cap) {
+    return {a.scale * LOG2E, cap ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E};
+}
 template <bool CAP>
 __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& r) {
     if (CAP) {
@@ -170,31 +231,40 @@ __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& r)
     return s * m.c;
 }
 
+// Masks shared by the kernels: how many keys at the front of a row every query sees (all of them without causality)
+__device__ __forceinline__ int seen_prefix(const AttendArgs& a, int b) {
+    if (!a.causal) return a.T;
+    return a.prefix != nullptr ? min(max(a.prefix[b], 0), a.T) : 0;
+}
+
+// Pipeline of the three kernels: two stages of LDS, each a 64-row tile of both streamed operands.  A stage's loads go out when
+// the stage in front of it is about to be used and have that tile's products to arrive in; one barrier per tile says both
+// that the tile is there and that nobody reads the stage that is filled next.
+template <int DH> constexpr int stage_bytes() { return 2 * tile_bytes<DH>(); }
+// waves per SIMD: what the registers of the accumulators and the stationary operand leave (512 / 2 at width 128)
+template <int DH> constexpr int occupancy() { return DH == 64 ? 3 : 2; }
+
 // ------------------------------------------------------------------------------ forward
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(AttendArgs a, unsigned short* __restrict__ out, unsigned short* __restrict__ rest, float* __restrict__ lse2) {
-    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>();
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * TB + TILE * 4];
-    unsigned char* Ks = smem;
-    unsigned char* Vs = smem + TB;
-    int* Kd = (int*)(smem + 2 * TB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(AttendArgs a, unsigned short* __restrict__ out, unsigned short* __restrict__ rest, float* __restrict__ lse2) {
+    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
+    __shared__ __attribute__((aligned(256))) int Kds[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ql = lane & 31, h = lane >> 5;
+    const FragAt<DH> frags(lane);
     const int head = blockIdx.x, b = blockIdx.y, hk = head / (a.Hq / a.Hkv);
     const int T = a.T, q0 = (gridDim.z - 1 - blockIdx.z) * BQ, qw0 = q0 + 32 * wave, q = qw0 + ql, qc = min(q, T - 1);
     const unsigned short* qbase = (const unsigned short*)a.q + b * a.qb + head * a.qh;
-    const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
-    const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
+    const TileDma<DH> kdma((const unsigned short*)a.k + b * a.kb + hk * a.kh, a.kt, T, a.D, tid);
+    const TileDma<DH> vdma((const unsigned short*)a.v + b * a.vb + hk * a.vh, a.vt, T, a.D, tid);
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int tiles = (T + TILE - 1) / TILE;
-    const int pre = a.causal ? (a.prefix != nullptr ? min(max(a.prefix[b], 0), T) : 0) : T;
+    const int pre = seen_prefix(a, b);
     const int lim = max(qc, pre - 1);                               // the last key that this lane's query sees
     const int qdoc = docs != nullptr ? docs[qc] : 0;
-    const ScoreMap sm{a.scale * LOG2E, CAP ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E};
+    const ScoreMap sm = score_map(a, CAP);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-
-    bf16x8 qf[KK];
-    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qdoc >= 0, qf);
 
     TileWalk walk;
     walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
@@ -202,62 +272,77 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(Atten
         walk.block = range_of(walk.rg, q0, BQ / 32, tiles);
         walk.wave = range_of(walk.rg, qw0, 1, tiles);
     }
-    walk.start(0, max(min(q0 + BQ, T), pre) / TILE + (max(min(q0 + BQ, T), pre) % TILE != 0));
+    walk.start(0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
 
+    int j = walk.next();
+    if (j < walk.end) {
+        kdma.fetch(smem, j * TILE, wave);
+        vdma.fetch(smem + TB, j * TILE, wave);
+        if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
+    }
+    bf16x8 qf[KK];
+    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qdoc >= 0, qf);
     floatx16 O[DI];
 #pragma unroll
     for (int di = 0; di < DI; ++di) zero16(O[di]);
     float m = NEG_BIG, l = 0.f;
-    Staged<DH> pk, pv;
-    int kd = 0;
-    int j = walk.next();
-    bool mine = walk.mine, whole = walk.whole;
-    if (j < walk.end) {
-        pk.fetch(kbase, a.kt, j * TILE, T, a.D, docs, tid);
-        pv.fetch(vbase, a.vt, j * TILE, T, a.D, docs, tid);
-        if (docs != nullptr && tid < TILE) kd = docs[min(j * TILE + tid, T - 1)];
-    }
-    while (j < walk.end) {
+    for (int stage = 0; j < walk.end; stage ^= 1) {
+        unsigned char* Ks = smem + stage * SB;
+        unsigned char* Vs = Ks + TB;
+        const int* Kd = Kds[stage];
+        tiles_landed();
         __syncthreads();
-        pk.stash(Ks, tid);
-        pv.stash(Vs, tid);
-        if (docs != nullptr && tid < TILE) Kd[tid] = kd;
-        __syncthreads();
+        if (walk.pad) {                                             // workgroup-uniform
+            clear_padding<DH>(Ks, Kd, tid);
+            clear_padding<DH>(Vs, Kd, tid);
+            __syncthreads();
+        }
         const int jt = j * TILE;
-        const bool go = mine && jt <= wave_last, same = whole, full = same && jt + TILE - 1 <= wave_least;
+        const bool go = walk.mine && jt <= wave_last, same = walk.whole, full = same && jt + TILE - 1 <= wave_least;
         j = walk.next();
-        mine = walk.mine; whole = walk.whole;
         if (j < walk.end) {
-            pk.fetch(kbase, a.kt, j * TILE, T, a.D, docs, tid);
-            pv.fetch(vbase, a.vt, j * TILE, T, a.D, docs, tid);
-            if (docs != nullptr && tid < TILE) kd = docs[min(j * TILE + tid, T - 1)];
+            kdma.fetch(smem + (stage ^ 1) * SB, j * TILE, wave);
+            vdma.fetch(smem + (stage ^ 1) * SB + TB, j * TILE, wave);
+            if (docs != nullptr && wave == 0) fetch_words(Kds[stage ^ 1], docs + j * TILE, T - j * TILE, lane);
         }
         if (!go) continue;                                          // wave-uniform
+        const FragAt<DH> fr = frags.fresh();
         floatx16 S[2];
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             zero16(S[t2]);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                S[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<DH>(Ks, 32 * t2 + ql, kk, h), qf[kk], S[t2], 0, 0, 0);
+                S[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Ks, t2, kk), qf[kk], S[t2], 0, 0, 0);
+        }
+        if (CAP || BIAS) {
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float rr;
+                    S[t2][r] = map_score<CAP>(sm, S[t2][r], rr);
+                    if (BIAS) S[t2][r] = fmaf(-slope2, fabsf((float)(q - jt - 4 * h) - (float)(32 * t2 + acc_row(r, 0))), S[t2][r]);
+                }
+        }
+        if (!full) {                                                // wave-uniform
+            const int to = lim - jt - 4 * h;                        // row acc_row(r, 0) of the tile is seen iff <= to (and of the document)
+            const int* kd4 = Kd + 4 * h;
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = 32 * t2 + acc_row(r, 0);
+                    const bool see = row <= to && (same || kd4[row] == qdoc);
+                    S[t2][r] = see ? S[t2][r] : MASKED;
+                }
         }
         float mx = NEG_BIG;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float rr;
-                float y = (CAP || BIAS) ? map_score<CAP>(sm, S[t2][r], rr) : S[t2][r];
-                if (BIAS) y = fmaf(-slope2, fabsf((float)(q - jt - 4 * h) - (float)(32 * t2 + acc_row(r, 0))), y);
-                if (!full) {                                        // wave-uniform
-                    const int key = 32 * t2 + acc_row(r, h);
-                    const bool see = jt + key <= lim && (same || Kd[key] == qdoc);
-                    y = see ? y : MASKED;
-                }
-                S[t2][r] = y;
-                mx = fmaxf(mx, y);
-            }
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[t2][r]);
         mx = xhalf_max(mx);
         const float c = (CAP || BIAS) ? 1.f : sm.c;                 // the scale rides the exponent's multiply-add where nothing else used it
         const float mn = fmaxf(m, mx * c);
@@ -289,7 +374,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(Atten
                 const bf16x8 pb = pack_regs(S[t2], s);
 #pragma unroll
                 for (int di = 0; di < DI; ++di)
-                    O[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<DH>(Vs, 32 * t2 + 16 * s + 4 * h, 32 * di, lane), pb,
+                    O[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Vs, t2, s, di), pb,
                                                                     O[di], 0, 0, 0);
             }
     }
@@ -317,29 +402,43 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_fwd_kernel(Atten
 
 // ------------------------------------------------------------------------------ dQ (query-stationary), and delta
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(AttendArgs a, const unsigned short* __restrict__ out, const unsigned short* __restrict__ rest,
+__global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(AttendArgs a, const unsigned short* __restrict__ out, const unsigned short* __restrict__ rest,
                                                                             const unsigned short* __restrict__ dout, const float* __restrict__ lse2,
-                                                                            float* __restrict__ delta, unsigned short* __restrict__ dq) {
-    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>();
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * TB + TILE * 4];
-    unsigned char* Ks = smem;
-    unsigned char* Vs = smem + TB;
-    int* Kd = (int*)(smem + 2 * TB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+                                                                            float2* __restrict__ stats, unsigned short* __restrict__ dq) {
+    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
+    __shared__ __attribute__((aligned(256))) int Kds[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ql = lane & 31, h = lane >> 5;
+    const FragAt<DH> frags(lane);
     const int head = blockIdx.x, b = blockIdx.y, hk = head / (a.Hq / a.Hkv);
     const int T = a.T, q0 = (gridDim.z - 1 - blockIdx.z) * BQ, qw0 = q0 + 32 * wave, q = qw0 + ql, qc = min(q, T - 1);
     const unsigned short* qbase = (const unsigned short*)a.q + b * a.qb + head * a.qh;
-    const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
-    const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
+    const TileDma<DH> kdma((const unsigned short*)a.k + b * a.kb + hk * a.kh, a.kt, T, a.D, tid);
+    const TileDma<DH> vdma((const unsigned short*)a.v + b * a.vb + hk * a.vh, a.vt, T, a.D, tid);
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int tiles = (T + TILE - 1) / TILE;
-    const int pre = a.causal ? (a.prefix != nullptr ? min(max(a.prefix[b], 0), T) : 0) : T;
+    const int pre = seen_prefix(a, b);
     const int lim = max(qc, pre - 1);
     const int qdoc = docs != nullptr ? docs[qc] : 0;
-    const ScoreMap sm{a.scale * LOG2E, CAP ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E};
+    const ScoreMap sm = score_map(a, CAP);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
     const long orow = (((long)b * T + qc) * a.Hq + head) * a.D;
+
+    TileWalk walk;
+    walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
+    if (docs != nullptr) {
+        walk.block = range_of(walk.rg, q0, BQ / 32, tiles);
+        walk.wave = range_of(walk.rg, qw0, 1, tiles);
+    }
+    walk.start(0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
+    const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
+    int j = walk.next();
+    if (j < walk.end) {
+        kdma.fetch(smem, j * TILE, wave);
+        vdma.fetch(smem + TB, j * TILE, wave);
+        if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
+    }
 
     bf16x8 qf[KK], dof[KK];
     load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qdoc >= 0, qf);
@@ -360,44 +459,30 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(Att
         for (int r = 0; r < 16; ++r) del = acc_row(r, h) == ql ? dd[r] : del;
         del = xhalf_sum(del);                                       // one half holds the diagonal element, the other zero
     }
-    if (h == 0 && q < T) delta[((long)b * a.Hq + head) * T + q] = del;
     const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
-
-    TileWalk walk;
-    walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
-    if (docs != nullptr) {
-        walk.block = range_of(walk.rg, q0, BQ / 32, tiles);
-        walk.wave = range_of(walk.rg, qw0, 1, tiles);
-    }
-    walk.start(0, max(min(q0 + BQ, T), pre) / TILE + (max(min(q0 + BQ, T), pre) % TILE != 0));
-    const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
+    if (h == 0 && q < T) stats[((long)b * a.Hq + head) * T + q] = make_float2(lse_q, del);
 
     floatx16 dQt[DI];
 #pragma unroll
     for (int di = 0; di < DI; ++di) zero16(dQt[di]);
-    Staged<DH> pk, pv;
-    int kd = 0;
-    int j = walk.next();
-    bool mine = walk.mine, whole = walk.whole;
-    if (j < walk.end) {
-        pk.fetch(kbase, a.kt, j * TILE, T, a.D, docs, tid);
-        pv.fetch(vbase, a.vt, j * TILE, T, a.D, docs, tid);
-        if (docs != nullptr && tid < TILE) kd = docs[min(j * TILE + tid, T - 1)];
-    }
-    while (j < walk.end) {
+    for (int stage = 0; j < walk.end; stage ^= 1) {
+        unsigned char* Ks = smem + stage * SB;
+        unsigned char* Vs = Ks + TB;
+        const int* Kd = Kds[stage];
+        tiles_landed();
         __syncthreads();
-        pk.stash(Ks, tid);
-        pv.stash(Vs, tid);
-        if (docs != nullptr && tid < TILE) Kd[tid] = kd;
-        __syncthreads();
+        if (walk.pad) {
+            clear_padding<DH>(Ks, Kd, tid);
+            clear_padding<DH>(Vs, Kd, tid);
+            __syncthreads();
+        }
         const int jt = j * TILE;
-        const bool go = mine && jt <= wave_last, same = whole;
+        const bool go = walk.mine && jt <= wave_last, same = walk.whole;
         j = walk.next();
-        mine = walk.mine; whole = walk.whole;
         if (j < walk.end) {
-            pk.fetch(kbase, a.kt, j * TILE, T, a.D, docs, tid);
-            pv.fetch(vbase, a.vt, j * TILE, T, a.D, docs, tid);
-            if (docs != nullptr && tid < TILE) kd = docs[min(j * TILE + tid, T - 1)];
+            kdma.fetch(smem + (stage ^ 1) * SB, j * TILE, wave);
+            vdma.fetch(smem + (stage ^ 1) * SB + TB, j * TILE, wave);
+            if (docs != nullptr && wave == 0) fetch_words(Kds[stage ^ 1], docs + j * TILE, T - j * TILE, lane);
         }
         if (!go) continue;
 #pragma unroll
@@ -405,34 +490,44 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(Att
             const int kt0 = jt + 32 * t2;
             if (kt0 > wave_last) continue;                          // wave-uniform
             const bool full = same && kt0 + 31 <= wave_least;
+            const FragAt<DH> fr = frags.fresh();
             floatx16 S, dP;
             zero16(S); zero16(dP);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<DH>(Ks, 32 * t2 + ql, kk, h), qf[kk], S, 0, 0, 0);
-                dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<DH>(Vs, 32 * t2 + ql, kk, h), dof[kk], dP, 0, 0, 0);
+                S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Ks, t2, kk), qf[kk], S, 0, 0, 0);
+                dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Vs, t2, kk), dof[kk], dP, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float rr = 0.f;
-                float y = map_score<CAP>(sm, S[r], rr);
-                if (BIAS) y = fmaf(-slope2, fabsf((float)(q - kt0 - 4 * h) - (float)acc_row(r, 0)), y);
-                const float p = fast_exp2(y - lse_q);
-                float ds = p * a.scale * (dP[r] - del);
-                if (CAP) ds *= 4.f * rr * (1.f - rr);
-                if (!full) {
-                    const int key = acc_row(r, h);
-                    const bool see = kt0 + key <= lim && (same || Kd[32 * t2 + key] == qdoc);
-                    ds = see ? ds : 0.f;
+                float rr = 0.f, e;
+                if (CAP || BIAS) {
+                    e = map_score<CAP>(sm, S[r], rr);
+                    if (BIAS) e = fmaf(-slope2, fabsf((float)(q - kt0 - 4 * h) - (float)acc_row(r, 0)), e);
+                    e -= lse_q;
+                } else {
+                    e = fmaf(S[r], sm.c, -lse_q);
                 }
+                float ds = fast_exp2(e) * a.scale * (dP[r] - del);
+                if (CAP) ds *= 4.f * rr * (1.f - rr);
                 S[r] = ds;
+            }
+            if (!full) {
+                const int to = lim - kt0 - 4 * h;
+                const int* kd4 = Kd + 32 * t2 + 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = acc_row(r, 0);
+                    const bool see = row <= to && (same || kd4[row] == qdoc);
+                    S[r] = see ? S[r] : 0.f;
+                }
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 dsb = pack_regs(S, s);
 #pragma unroll
                 for (int di = 0; di < DI; ++di)
-                    dQt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<DH>(Ks, 32 * t2 + 16 * s + 4 * h, 32 * di, lane), dsb,
+                    dQt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Ks, t2, s, di), dsb,
                                                                       dQt[di], 0, 0, 0);
             }
         }
@@ -442,27 +537,25 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_q_kernel(Att
 
 // ------------------------------------------------------------------------------ dK / dV (key-stationary, no atomics)
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
-                                                                             const float* __restrict__ lse2, const float* __restrict__ delta,
-                                                                             unsigned short* __restrict__ dk, unsigned short* __restrict__ dv) {
-    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>();
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * TB + 3 * TILE * 4];
-    unsigned char* Qs = smem;
-    unsigned char* Os = smem + TB;
-    float* lse_s = (float*)(smem + 2 * TB);
-    float* del_s = lse_s + TILE;
-    int* Qd = (int*)(del_s + TILE);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__global__ __launch_bounds__(256, 2) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+                                                               const float2* __restrict__ stats, unsigned short* __restrict__ dk,
+                                                               unsigned short* __restrict__ dv) {
+    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
+    __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
+    __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kl = lane & 31, h = lane >> 5;
+    const FragAt<DH> frags(lane);
     const int hk = blockIdx.x, b = blockIdx.y, group = a.Hq / a.Hkv;
     const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * wave, key = kw0 + kl, keyc = min(key, T - 1);
     const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
     const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int tiles = (T + TILE - 1) / TILE;
-    const int pre = a.causal ? (a.prefix != nullptr ? min(max(a.prefix[b], 0), T) : 0) : T;
+    const int pre = seen_prefix(a, b);
     const int kdoc = docs != nullptr ? docs[keyc] : 0;
-    const ScoreMap sm{a.scale * LOG2E, CAP ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E};
+    const ScoreMap sm = score_map(a, CAP);
 
     bf16x8 kf[KK], vf[KK];
     load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kdoc >= 0, kf);
@@ -482,79 +575,87 @@ __global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attend_bwd_kv_kernel(At
 
     for (int g = 0; g < group; ++g) {
         const int head = hk * group + g;
-        const unsigned short* qbase = (const unsigned short*)a.q + b * a.qb + head * a.qh;
-        const unsigned short* dobase = dout + ((long)b * T * a.Hq + head) * a.D;
-        const float* lse_b = lse2 + ((long)b * a.Hq + head) * T;
-        const float* del_b = delta + ((long)b * a.Hq + head) * T;
-        const long ors = (long)a.Hq * a.D;
+        const TileDma<DH> qdma((const unsigned short*)a.q + b * a.qb + head * a.qh, a.qt, T, a.D, tid);
+        const TileDma<DH> odma(dout + ((long)b * T * a.Hq + head) * a.D, (long)a.Hq * a.D, T, a.D, tid);
+        const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
         const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-        Staged<DH> pq, po;
-        float pl = 0.f, pd = 0.f;
-        int pdoc = 0;
         walk.start(first, tiles);
         int j = walk.next();
-        bool mine = walk.mine, whole = walk.whole;
-#define DPA_FETCH_Q()                                                                  \
-    if (j < walk.end) {                                                                \
-        pq.fetch(qbase, a.qt, j * TILE, T, a.D, docs, tid);                            \
-        po.fetch(dobase, ors, j * TILE, T, a.D, docs, tid);                            \
-        if (tid < TILE) {                                                              \
-            const int qi = j * TILE + tid;                                             \
-            pl = qi < T ? lse_b[qi] : 1.0e30f;                                         \
-            pd = qi < T ? del_b[qi] : 0.f;                                             \
-            pdoc = docs != nullptr && qi < T ? docs[qi] : 0;                           \
-        }                                                                              \
+#define DPA_FETCH_Q(S_)                                                                                                  \
+    if (j < walk.end) {                                                                                                  \
+        qdma.fetch(smem + (S_) * SB, j * TILE, wave);                                                                    \
+        odma.fetch(smem + (S_) * SB + TB, j * TILE, wave);                                                               \
+        if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2L * (T - j * TILE - 32 * wave), lane);  \
+        else if (wave == 2 && docs != nullptr) fetch_words(Qds[S_], docs + j * TILE, T - j * TILE, lane);                \
     }
-        DPA_FETCH_Q()
-        while (j < walk.end) {
+        __syncthreads();                                            // the stages are free of the head before
+        DPA_FETCH_Q(0)
+        for (int stage = 0; j < walk.end; stage ^= 1) {
+            unsigned char* Qs = smem + stage * SB;
+            unsigned char* Os = Qs + TB;
+            const float2* lds_s = lds_ss[stage];
+            const int* Qd = Qds[stage];
+            tiles_landed();
             __syncthreads();
-            pq.stash(Qs, tid);
-            po.stash(Os, tid);
-            if (tid < TILE) { lse_s[tid] = pl; del_s[tid] = pd; Qd[tid] = pdoc; }
-            __syncthreads();
+            if (walk.pad) {
+                clear_padding<DH>(Qs, Qd, tid);
+                clear_padding<DH>(Os, Qd, tid);
+                __syncthreads();
+            }
             const int jt = j * TILE;
-            const bool go = mine && (jt + TILE - 1 >= kw0 || kw0 < pre), same = whole;
+            const bool go = walk.mine && (jt + TILE - 1 >= kw0 || kw0 < pre), same = walk.whole;
             j = walk.next();
-            mine = walk.mine; whole = walk.whole;
-            DPA_FETCH_Q()
+            DPA_FETCH_Q(stage ^ 1)
             if (!go) continue;                                      // wave-uniform
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2) {
                 const int qt0 = jt + 32 * t2;
                 if (qt0 + 31 < kw0 && kw0 >= pre) continue;         // wave-uniform
-                const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre);
+                const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre) && qt0 + 32 <= T;
+                const FragAt<DH> fr = frags.fresh();
                 floatx16 S, dP;
                 zero16(S); zero16(dP);
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
-                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<DH>(Qs, 32 * t2 + kl, kk, h), kf[kk], S, 0, 0, 0);
-                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<DH>(Os, 32 * t2 + kl, kk, h), vf[kk], dP, 0, 0, 0);
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Qs, t2, kk), kf[kk], S, 0, 0, 0);
+                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Os, t2, kk), vf[kk], dP, 0, 0, 0);
                 }
+                const float2* ld4 = lds_s + 32 * t2 + 4 * h;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int qr = 32 * t2 + acc_row(r, h);
-                    float rr = 0.f;
-                    float y = map_score<CAP>(sm, S[r], rr);
-                    if (BIAS) y = fmaf(-slope2, fabsf((float)(qt0 + 4 * h - key) + (float)acc_row(r, 0)), y);
-                    float p = fast_exp2(y - lse_s[qr]);
-                    float ds = p * a.scale * (dP[r] - del_s[qr]);
-                    if (CAP) ds *= 4.f * rr * (1.f - rr);
-                    if (!full) {
-                        const bool see = jt + qr >= key_from && (same || Qd[qr] == kdoc);
-                        p = see ? p : 0.f;
-                        ds = see ? ds : 0.f;
+                    const int row = acc_row(r, 0);
+                    float rr = 0.f, e;
+                    if (CAP || BIAS) {
+                        e = map_score<CAP>(sm, S[r], rr);
+                        if (BIAS) e = fmaf(-slope2, fabsf((float)(qt0 + 4 * h - key) + (float)row), e);
+                        e -= ld4[row].x;
+                    } else {
+                        e = fmaf(S[r], sm.c, -ld4[row].x);
                     }
+                    const float p = fast_exp2(e);
+                    float ds = p * a.scale * (dP[r] - ld4[row].y);
+                    if (CAP) ds *= 4.f * rr * (1.f - rr);
                     S[r] = p;
                     dP[r] = ds;
+                }
+                if (!full) {
+                    const int from = key_from - qt0 - 4 * h, past = T - qt0 - 4 * h;   // row acc_row(r, 0) sees this lane's key iff from <= row < past
+                    const int* qd4 = Qd + 32 * t2 + 4 * h;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = acc_row(r, 0);
+                        const bool see = row >= from && row < past && (same || qd4[row] == kdoc);
+                        S[r] = see ? S[r] : 0.f;
+                        dP[r] = see ? dP[r] : 0.f;
+                    }
                 }
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const bf16x8 pb = pack_regs(S, s), dsb = pack_regs(dP, s);
-                    const int rowbase = 32 * t2 + 16 * s + 4 * h;
 #pragma unroll
                     for (int di = 0; di < DI; ++di) {
-                        dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<DH>(Os, rowbase, 32 * di, lane), pb, dVt[di], 0, 0, 0);
-                        dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<DH>(Qs, rowbase, 32 * di, lane), dsb, dKt[di], 0, 0, 0);
+                        dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Os, t2, s, di), pb, dVt[di], 0, 0, 0);
+                        dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Qs, t2, s, di), dsb, dKt[di], 0, 0, 0);
                     }
                 }
             }
@@ -574,12 +675,12 @@ void fwd_of(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t
                        (unsigned short*)rest, lse2);
 }
 template <int DH, bool CAP, bool BIAS>
-void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
+void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv, hipStream_t st) {
     const int blocks = (a.T + BQ - 1) / BQ;
     hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
-                       (const unsigned short*)rest, (const unsigned short*)dout, lse2, delta, (unsigned short*)dq);
+                       (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
     hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout,
-                       lse2, delta, (unsigned short*)dk, (unsigned short*)dv);
+                       (const float2*)stats, (unsigned short*)dk, (unsigned short*)dv);
 }
 
 }  // namespace
@@ -604,8 +705,8 @@ void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t 
 
 void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) { DPA_ATTEND_PICK(fwd_of, a, out, rest, lse2, st); }
 
-void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t st) {
-    DPA_ATTEND_PICK(bwd_of, a, out, rest, dout, lse2, delta, dq, dk, dv, st);
+void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv, hipStream_t st) {
+    DPA_ATTEND_PICK(bwd_of, a, out, rest, dout, lse2, stats, dq, dk, dv, st);
 }
 
 }  // namespace dpa

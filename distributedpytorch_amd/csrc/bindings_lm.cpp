@@ -32,10 +32,10 @@ OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor()
 Tensor bare(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 Tensor flat16(const Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
-// last axis contiguous, every row on 16 bytes
+// last axis contiguous, every row on 16 bytes, 64 tokens within 32-bit offsets
 Tensor rows16(const Tensor& t) {
     bool ok = on16(t) && (t.size(-1) <= 1 || t.stride(-1) == 1);
-    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && (i != 1 || t.stride(i) < (1 << 23))));
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -57,7 +57,8 @@ dpa::AttendArgs attend_args(const Tensor& q, const Tensor& k, const Tensor& v, b
     const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(2);
     TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(1) == T && k.size(3) == D, "attend: shapes");
     TORCH_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && D >= 8 && D % 8 == 0 && D <= 128, "attend: heads");
-    TORCH_CHECK(B <= 65535 && T <= (1 << 22) && Hq <= 65535, "attend: oversized problem");
+    TORCH_CHECK(B <= 65535 && T <= (1 << 22) && Hq <= 65535 && (int64_t)Hq * D < (1 << 23), "attend: oversized problem");
+    for (const Tensor* t : {&q, &k, &v}) TORCH_CHECK(T <= 1 || t->stride(1) < (1 << 23), "attend: token stride");
     TORCH_CHECK(scale > 1e-12 && scale < 1e12 && softcap >= 0.0 && softcap < 1e12, "attend: scale, softcap");
     dpa::AttendArgs a{};
     a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
@@ -118,8 +119,8 @@ std::vector<Tensor> attend_bwd(const Tensor& q, const Tensor& k, const Tensor& v
         CHECK_FLAT16((*ranges), q, at::kInt);
         a.ranges = (const int4*)ranges->data_ptr();
     }
-    Tensor delta = torch::empty_like(lse2);
-    dpa::attend_bwd(a, out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    Tensor stats = torch::empty({a.B, a.Hq, a.T, 2}, lse2.options());
+    dpa::attend_bwd(a, out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), stats.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                     cur_stream());
     return {dq, dk, dv};
 }

@@ -99,7 +99,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
         raise TypeError(f"attention: bf16 on the GPU, got {q.dtype}")
     if D % 8 or D > 128:
         raise ValueError(f"attention: head dimension {D}: a multiple of 8 up to 128 on the GPU")
-    if B > 65535 or Hq > 65535 or T > 1 << 22:
-        raise ValueError("attention: at most 65,535 rows, 65,535 heads and 4,194,304 tokens in a row")
+    if B > 65535 or Hq > 65535 or Hq * D >= 1 << 23 or T > 1 << 22:
+        raise ValueError("attention: at most 65,535 rows, 65,535 heads, 2^23 - 1 channels and 2^22 tokens in a row")
     slopes, documents, prefix = (t if t is None else t.contiguous() for t in (slopes, documents, prefix))
     return _ext.load().attention_ex(q, k, v, bool(causal), scale, softcap, slopes, documents, prefix)
