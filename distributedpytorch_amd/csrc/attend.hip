@@ -536,10 +536,13 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
 }
 
 // ------------------------------------------------------------------------------ dK / dV (key-stationary, no atomics)
+// A key head's gradient sums over its group of query heads.  Where that leaves few workgroups (kv_parts below) the group is
+// cut: a workgroup takes `heads` of its query heads and writes its sums in fp32 to part [part][B, T, Hkv, D], dK and then dV,
+// and fold_parts_kernel adds the parts in order.
 template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+__global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
                                                                const float2* __restrict__ stats, unsigned short* __restrict__ dk,
-                                                               unsigned short* __restrict__ dv) {
+                                                               unsigned short* __restrict__ dv, float* __restrict__ part, int heads) {
     constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
     __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_kernel(AttendArgs a, con
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kl = lane & 31, h = lane >> 5;
     const FragAt<DH> frags(lane);
-    const int hk = blockIdx.x, b = blockIdx.y, group = a.Hq / a.Hkv;
+    const int hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
     const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * wave, key = kw0 + kl, keyc = min(key, T - 1);
     const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
     const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
@@ -573,8 +576,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_kernel(AttendArgs a, con
     const int first = k0 < pre ? 0 : k0 / TILE;                     // in front of the first key only a prefix key is seen
     const int key_from = key < pre ? -(1 << 30) : key;              // the first query that sees this lane's key
 
-    for (int g = 0; g < group; ++g) {
-        const int head = hk * group + g;
+    for (int head = hq0; head < hq0 + heads; ++head) {
         const TileDma<DH> qdma((const unsigned short*)a.q + b * a.qb + head * a.qh, a.qt, T, a.D, tid);
         const TileDma<DH> odma(dout + ((long)b * T * a.Hq + head) * a.D, (long)a.Hq * a.D, T, a.D, tid);
         const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
@@ -662,10 +664,37 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_kernel(AttendArgs a, con
         }
 #undef DPA_FETCH_Q
     }
-    if (key < T) {
+    if (key < T && part != nullptr) {
+        const long row = (((long)b * T + key) * a.Hkv + hk) * a.D, n = (long)a.B * T * a.Hkv * a.D;
+        float* to = part + (long)(hq0 / heads % (a.Hq / a.Hkv / heads)) * 2 * n + row;
+#pragma unroll
+        for (int di = 0; di < DI; ++di)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * di + 8 * g + 4 * h;
+                if (d < a.D) {
+                    *(float4*)(to + d) = make_float4(dKt[di][4 * g], dKt[di][4 * g + 1], dKt[di][4 * g + 2], dKt[di][4 * g + 3]);
+                    *(float4*)(to + n + d) = make_float4(dVt[di][4 * g], dVt[di][4 * g + 1], dVt[di][4 * g + 2], dVt[di][4 * g + 3]);
+                }
+            }
+    } else if (key < T) {
         const long row = (((long)b * T + key) * a.Hkv + hk) * a.D;
         store_cols<DH>(dk + row, dKt, kdoc >= 0 ? 1.f : 0.f, h, a.D);
         store_cols<DH>(dv + row, dVt, kdoc >= 0 ? 1.f : 0.f, h, a.D);
+    }
+}
+
+// dk, dv [n] = the sum of their parts [parts][2][n] in order, rounded once (n a multiple of 8)
+__global__ __launch_bounds__(256) void fold_parts_kernel(const float* __restrict__ part, int parts, long n, unsigned short* __restrict__ dk,
+                                                         unsigned short* __restrict__ dv) {
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < 2 * n; i += (long)gridDim.x * 256 * 8) {
+        float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const float4 x = *(const float4*)(part + 2 * n * p + i), y = *(const float4*)(part + 2 * n * p + i + 4);
+            s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w; s[4] += y.x; s[5] += y.y; s[6] += y.z; s[7] += y.w;
+        }
+        *(uint4*)(i < n ? dk + i : dv + i - n) = pack8(s);
     }
 }
 
@@ -675,12 +704,18 @@ void fwd_of(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t
                        (unsigned short*)rest, lse2);
 }
 template <int DH, bool CAP, bool BIAS>
-void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv, hipStream_t st) {
+void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv,
+            float* part, hipStream_t st) {
     const int blocks = (a.T + BQ - 1) / BQ;
     hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
                        (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
-    hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout,
-                       (const float2*)stats, (unsigned short*)dk, (unsigned short*)dv);
+    const int parts = part != nullptr ? attend_kv_parts(a) : 1, heads = a.Hq / a.Hkv / parts;
+    hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout,
+                       (const float2*)stats, (unsigned short*)dk, (unsigned short*)dv, part, heads);
+    if (part != nullptr) {
+        const long n = (long)a.B * a.T * a.Hkv * a.D, grid = (2 * n / 8 + 255) / 256;
+        hipLaunchKernelGGL(fold_parts_kernel, dim3((unsigned)(grid > 8192 ? 8192 : grid)), dim3(256), 0, st, part, parts, n, (unsigned short*)dk, (unsigned short*)dv);
+    }
 }
 
 }  // namespace
@@ -705,8 +740,19 @@ void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t 
 
 void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) { DPA_ATTEND_PICK(fwd_of, a, out, rest, lse2, st); }
 
-void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv, hipStream_t st) {
-    DPA_ATTEND_PICK(bwd_of, a, out, rest, dout, lse2, stats, dq, dk, dv, st);
+// Query heads of a group in how many workgroups: the fewest that give 1024 of them (4 per CU: their work differs by where
+// their keys stand), or one head each.  PARTS_FIGURES
+int attend_kv_parts(const AttendArgs& a) {
+    const int group = a.Hq / a.Hkv;
+    const long wgs = (long)a.Hkv * a.B * ((a.T + BQ - 1) / BQ);
+    for (int p = 1; p < group; ++p)
+        if (group % p == 0 && wgs * p >= 1024) return p;
+    return group;
+}
+
+void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv,
+                float* part, hipStream_t st) {
+    DPA_ATTEND_PICK(bwd_of, a, out, rest, dout, lse2, stats, dq, dk, dv, part, st);
 }
 
 }  // namespace dpa

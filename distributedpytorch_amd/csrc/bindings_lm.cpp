@@ -120,8 +120,11 @@ std::vector<Tensor> attend_bwd(const Tensor& q, const Tensor& k, const Tensor& v
         a.ranges = (const int4*)ranges->data_ptr();
     }
     Tensor stats = torch::empty({a.B, a.Hq, a.T, 2}, lse2.options());
+    const int parts = dpa::attend_kv_parts(a);
+    Tensor part;
+    if (parts > 1) part = torch::empty({parts, 2, dk.numel()}, lse2.options());
     dpa::attend_bwd(a, out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse2.data_ptr<float>(), stats.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                    cur_stream());
+                    parts > 1 ? part.data_ptr<float>() : nullptr, cur_stream());
     return {dq, dk, dv};
 }
 

@@ -257,8 +257,11 @@ void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t 
 // lse2 [B, Hq, T]: log2 of the row's sum of 2^score (1e30 for a row that sees nothing)
 // rest (or nullptr): what the rounding of out to bf16 took away, itself in bf16; backward needs it
 void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st);
-// out, rest, dout, dq [B,T,Hq,D], dk, dv [B,T,Hkv,D] contiguous; stats [B, Hq, T, 2] fp32 is scratch
-void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv, hipStream_t st);
+// out, rest, dout, dq [B,T,Hq,D], dk, dv [B,T,Hkv,D] contiguous; stats [B, Hq, T, 2] fp32 is scratch, and so is
+// part [attend_kv_parts][2][B, T, Hkv, D] fp32, nullptr where that is 1
+int attend_kv_parts(const AttendArgs& a);
+void attend_bwd(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv,
+                float* part, hipStream_t st);
 // head norms and rotation over a packed projection [tokens, (Hq + 2 Hkv) * D] bf16 (heads.hip)
 struct HeadsArgs {
     const void* qkv;
