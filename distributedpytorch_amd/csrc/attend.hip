@@ -55,18 +55,6 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const int* __restrict__
     if (lane == 0) ranges[(long)blockIdx.y * tiles + t] = make_int4(lo, hi, lo2, hi2);
 }
 
-// document range of rows r0 .. r0 + 32 n - 1 (r0 a multiple of 32, ends past the last tile left out)
-__device__ __forceinline__ DocRange range_of(const int4* rg, int r0, int n, int tiles) {
-    DocRange d{0x7fffffff, -0x7fffffff};
-    for (int i = 0; i < n; ++i) {
-        const int g = (r0 >> 5) + i;
-        if ((g >> 1) >= tiles) break;
-        const int4 v = rg[g >> 1];
-        d = merge(d, (g & 1) ? DocRange{v.z, v.w} : DocRange{v.x, v.y});
-    }
-    return d;
-}
-
 // Walks the 64-row tiles first .. end - 1 that a workgroup's rows can share a document with.  `mine` / `whole`: whether the
 // wave's own 32 rows meet the current tile, and whether every pair of the two is of one document.
 struct TileWalk {
@@ -76,15 +64,11 @@ struct TileWalk {
     unsigned long long todo, mine_bits, whole_bits, pad_bits;
     bool mine, whole, pad;                // pad: some of the tile's rows are padding
 
-    __device__ __forceinline__ void look() {
+    __device__ __forceinline__ void look(const int4& v) {          // v: this lane's entry (of a tile in range)
         const int lane = threadIdx.x & 63, t = base + lane;
         bool a = t < end, b = true, c = true, p = false;
         if (rg != nullptr) {
-            DocRange d{0x7fffffff, -0x7fffffff};
-            if (a) {
-                const int4 v = rg[t];
-                d = merge(DocRange{v.x, v.y}, DocRange{v.z, v.w});
-            }
+            const DocRange d = merge(DocRange{v.x, v.y}, DocRange{v.z, v.w});
             a = a && meets(d, block);
             b = meets(d, wave);
             c = same_doc(d, wave);
@@ -92,13 +76,35 @@ struct TileWalk {
         }
         todo = __ballot(a); mine_bits = __ballot(b); whole_bits = __ballot(c); pad_bits = __ballot(p);
     }
-    __device__ __forceinline__ void start(int first, int end_) { base = first; end = end_; look(); }
+    __device__ __forceinline__ int4 entry() const {
+        const int t = base + (int)(threadIdx.x & 63);
+        return rg != nullptr ? rg[min(t, end - 1)] : make_int4(0, 0, 0, 0);
+    }
+    // Rows row0 .. row0 + 127 (a multiple of 128; the wave's own are 32 w ..) against tiles first .. end_ - 1, end_ > first.  One
+    // round of loads: the entries of the rows' own two tiles and the first 64 of the walk go out together.
+    __device__ __forceinline__ void open(const int4* rg_, int tiles, int row0, int w, int first, int end_) {
+        rg = rg_; base = first; end = end_;
+        int4 v = entry();
+        if (rg != nullptr) {
+            const int t0 = row0 / TILE;
+            const int4 o = rg[min(t0 + (int)(threadIdx.x & 1), tiles - 1)];
+            const bool two = t0 + 1 < tiles;
+            const auto lane_of = [](int x, int l) { return __builtin_amdgcn_readlane(x, l); };
+            const int lo = min(o.x, o.z), hi = max(o.y, o.w), lo1 = lane_of(lo, 1), hi1 = lane_of(hi, 1);
+            block = merge(DocRange{lane_of(lo, 0), lane_of(hi, 0)}, DocRange{two ? lo1 : 0x7fffffff, two ? hi1 : -0x7fffffff});
+            const bool there = w < 2 || two;
+            const int wlo = lane_of((w & 1) ? o.z : o.x, w >> 1), whi = lane_of((w & 1) ? o.w : o.y, w >> 1);
+            wave = {there ? wlo : 0x7fffffff, there ? whi : -0x7fffffff};
+        }
+        look(v);
+    }
+    __device__ __forceinline__ void restart(int first) { base = first; look(entry()); }
     // the next tile, or `end` when there is none
     __device__ __forceinline__ int next() {
         while (todo == 0) {
             base += 64;
             if (base >= end) { base = end; return end; }
-            look();
+            look(entry());
         }
         const int bit = __ffsll((long long)todo) - 1;
         todo &= todo - 1;
@@ -189,15 +195,24 @@ struct FragAt {
     }
 };
 
-// this lane's half of one row as MFMA fragments, zero from column D on (and everywhere unless `live`)
+// this lane's half of one row as MFMA fragments, zero from column D on
 template <int DH>
-__device__ __forceinline__ void load_frags(const unsigned short* row, int h, int D, bool live, bf16x8 (&f)[DH / 16]) {
+__device__ __forceinline__ void load_frags(const unsigned short* row, int h, int D, bf16x8 (&f)[DH / 16]) {
 #pragma unroll
     for (int kk = 0; kk < DH / 16; ++kk) {
         const int col = 16 * kk + 8 * h;
         u32x4 v = {0, 0, 0, 0};
-        if (live && col < D) v = *(const u32x4*)(row + col);
+        if (col < D) v = *(const u32x4*)(row + col);
         f[kk] = __builtin_bit_cast(bf16x8, v);
+    }
+}
+// ... and zero all over where the row is padding (apart from the loads: they need not wait for the document number)
+template <int DH>
+__device__ __forceinline__ void zero_unless(bool live, bf16x8 (&f)[DH / 16]) {
+#pragma unroll
+    for (int kk = 0; kk < DH / 16; ++kk) {
+        const u32x4 v = __builtin_bit_cast(u32x4, f[kk]);
+        f[kk] = __builtin_bit_cast(bf16x8, live ? v : u32x4{0, 0, 0, 0});
     }
 }
 
@@ -258,6 +273,8 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
     const unsigned short* qbase = (const unsigned short*)a.q + b * a.qb + head * a.qh;
     const TileDma<DH> kdma((const unsigned short*)a.k + b * a.kb + hk * a.kh, a.kt, T, a.D, tid);
     const TileDma<DH> vdma((const unsigned short*)a.v + b * a.vb + hk * a.vh, a.vt, T, a.D, tid);
+    bf16x8 qf[KK];
+    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qf);
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int tiles = (T + TILE - 1) / TILE;
     const int pre = seen_prefix(a, b);
@@ -267,12 +284,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
 
     TileWalk walk;
-    walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
-    if (docs != nullptr) {
-        walk.block = range_of(walk.rg, q0, BQ / 32, tiles);
-        walk.wave = range_of(walk.rg, qw0, 1, tiles);
-    }
-    walk.start(0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
+    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
 
     int j = walk.next();
@@ -281,8 +293,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         vdma.fetch(smem + TB, j * TILE, wave);
         if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
     }
-    bf16x8 qf[KK];
-    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qdoc >= 0, qf);
+    zero_unless<DH>(qdoc >= 0, qf);
     floatx16 O[DI];
 #pragma unroll
     for (int di = 0; di < DI; ++di) zero16(O[di]);
@@ -416,6 +427,10 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const unsigned short* qbase = (const unsigned short*)a.q + b * a.qb + head * a.qh;
     const TileDma<DH> kdma((const unsigned short*)a.k + b * a.kb + hk * a.kh, a.kt, T, a.D, tid);
     const TileDma<DH> vdma((const unsigned short*)a.v + b * a.vb + hk * a.vh, a.vt, T, a.D, tid);
+    const long orow = (((long)b * T + qc) * a.Hq + head) * a.D;
+    bf16x8 qf[KK], dof[KK];
+    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qf);
+    load_frags<DH>(dout + orow, h, a.D, dof);
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int tiles = (T + TILE - 1) / TILE;
     const int pre = seen_prefix(a, b);
@@ -423,15 +438,10 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const int qdoc = docs != nullptr ? docs[qc] : 0;
     const ScoreMap sm = score_map(a, CAP);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-    const long orow = (((long)b * T + qc) * a.Hq + head) * a.D;
+    const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
 
     TileWalk walk;
-    walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
-    if (docs != nullptr) {
-        walk.block = range_of(walk.rg, q0, BQ / 32, tiles);
-        walk.wave = range_of(walk.rg, qw0, 1, tiles);
-    }
-    walk.start(0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
+    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
     int j = walk.next();
     if (j < walk.end) {
@@ -440,26 +450,24 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
         if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
     }
 
-    bf16x8 qf[KK], dof[KK];
-    load_frags<DH>(qbase + (long)qc * a.qt, h, a.D, qdoc >= 0, qf);
-    load_frags<DH>(dout + orow, h, a.D, qdoc >= 0, dof);
     float del;
     {
-        bf16x8 of[KK];
-        load_frags<DH>(out + orow, h, a.D, qdoc >= 0, of);
+        bf16x8 of[KK], rf[KK];
+        load_frags<DH>(out + orow, h, a.D, of);
+        load_frags<DH>(rest + orow, h, a.D, rf);
+        zero_unless<DH>(qdoc >= 0, qf);
+        zero_unless<DH>(qdoc >= 0, dof);                            // out and rest of a padded row are zeros already
         floatx16 dd;
         zero16(dd);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) dd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(of[kk], dof[kk], dd, 0, 0, 0);
-        load_frags<DH>(rest + orow, h, a.D, qdoc >= 0, of);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) dd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(of[kk], dof[kk], dd, 0, 0, 0);
+        for (int kk = 0; kk < KK; ++kk) dd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[kk], dof[kk], dd, 0, 0, 0);
         del = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) del = acc_row(r, h) == ql ? dd[r] : del;
         del = xhalf_sum(del);                                       // one half holds the diagonal element, the other zero
     }
-    const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
     if (h == 0 && q < T) stats[((long)b * a.Hq + head) * T + q] = make_float2(lse_q, del);
 
     floatx16 dQt[DI];
@@ -561,19 +569,17 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
     const ScoreMap sm = score_map(a, CAP);
 
     bf16x8 kf[KK], vf[KK];
-    load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kdoc >= 0, kf);
-    load_frags<DH>(vbase + (long)keyc * a.vt, h, a.D, kdoc >= 0, vf);
+    load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kf);
+    load_frags<DH>(vbase + (long)keyc * a.vt, h, a.D, vf);
+    zero_unless<DH>(kdoc >= 0, kf);
+    zero_unless<DH>(kdoc >= 0, vf);
     floatx16 dKt[DI], dVt[DI];
 #pragma unroll
     for (int di = 0; di < DI; ++di) { zero16(dKt[di]); zero16(dVt[di]); }
 
-    TileWalk walk;
-    walk.rg = docs != nullptr ? a.ranges + (long)b * tiles : nullptr;
-    if (docs != nullptr) {
-        walk.block = range_of(walk.rg, k0, BQ / 32, tiles);
-        walk.wave = range_of(walk.rg, kw0, 1, tiles);
-    }
     const int first = k0 < pre ? 0 : k0 / TILE;                     // in front of the first key only a prefix key is seen
+    TileWalk walk;
+    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, k0, wave, first, tiles);
     const int key_from = key < pre ? -(1 << 30) : key;              // the first query that sees this lane's key
 
     for (int head = hq0; head < hq0 + heads; ++head) {
@@ -581,7 +587,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
         const TileDma<DH> odma(dout + ((long)b * T * a.Hq + head) * a.D, (long)a.Hq * a.D, T, a.D, tid);
         const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
         const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-        walk.start(first, tiles);
+        if (head > hq0) walk.restart(first);
         int j = walk.next();
 #define DPA_FETCH_Q(S_)                                                                                                  \
     if (j < walk.end) {                                                                                                  \
