@@ -119,24 +119,27 @@ struct TileWalk {
 // other operand of every product that sums over them is zero there).  Completion: tiles_landed(), then a barrier.
 template <int DH>
 struct TileDma {
-    const unsigned short* base;          // row 0
-    long rs;                             // row stride, elements
+    const unsigned char* base;           // row 0
+    unsigned step;                       // bytes of 64 rows' strides
+    unsigned whole, last;                // what a tile may read: a full one's bytes, the last one's
     unsigned off;                        // this lane's bytes in the tile's first rows
-    int T, D;
-    __device__ __forceinline__ TileDma(const unsigned short* g, long rs_, int T_, int D_, int tid) : base(g), rs(rs_), T(T_), D(D_) {
+    __device__ __forceinline__ TileDma(const unsigned short* g, long rs, int T, int D, int tid) : base((const unsigned char*)g) {
         constexpr int CPR = DH / 8;
         const int row = tid / CPR, slot = tid % CPR;
         const int key = DH == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
-        off = (unsigned)(row * rs * 2) + 2 * min((slot ^ key) * 8, D - 8);
+        const unsigned rb = (unsigned)rs * 2;
+        off = row * rb + 2 * min((slot ^ key) * 8, D - 8);
+        step = 64 * rb;
+        whole = 63 * rb + 2 * D;
+        last = ((T - 1) % TILE) * rb + 2 * D;
     }
-    __device__ __forceinline__ void fetch(unsigned char* lds, int r0, int wave) const {
-        constexpr int RSTEP = 256 / (DH / 8);                        // rows a workgroup's instruction covers: a multiple of 16, so `key` repeats
-        const u32x4 words = buffer_words(base + (long)r0 * rs, (unsigned)(((min(TILE, T - r0) - 1) * rs + D) * 2));
+    __device__ __forceinline__ void fetch(unsigned char* lds, int j, bool is_last, int wave) const {
+        const u32x4 words = buffer_words(base + (unsigned long long)step * (unsigned)j, is_last ? last : whole);
         unsigned o = off;
         asm volatile("" : "+v"(o));                                  // the sums below are formed here, not kept across the loop
 #pragma unroll
-        for (int i = 0; i < DH / 32; ++i)
-            dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + (unsigned)(i * RSTEP * rs * 2));
+        for (int i = 0; i < DH / 32; ++i)                            // 256 / (DH / 8) rows each: a multiple of 16, so `key` repeats
+            dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + i * (step / (DH / 32)));
     }
 };
 // 64 words (documents, statistics) into LDS by one wave, a word a lane; zeros from word `n` on
@@ -169,28 +172,29 @@ __device__ __forceinline__ void clear_padding(unsigned char* lds, const int* doc
 // put the backward kernels past their budget.
 template <int DH>
 struct FragAt {
-    int row, tr;
+    unsigned row, tr;
     __device__ __forceinline__ explicit FragAt(int lane) {
         const int r = lane & 31, h = lane >> 5, tq = (lane & 15) >> 2, tp = lane & 3, gi = (lane >> 4) & 1;
         row = img_off<DH>(r, 8 * h);
         tr = img_off<DH>(4 * h + tq, 16 * gi + 4 * tp);
     }
-    // a copy whose offsets the compiler takes for new ones: it forms the XORs where they are used instead of keeping all of
-    // them in registers across the loop
-    __device__ __forceinline__ FragAt fresh() const {
+    // the same in the image `base` bytes on (a multiple of a row).  The compiler takes the offsets for new ones: it forms the
+    // XORs where they are used instead of keeping all of them in registers across the loop
+    __device__ __forceinline__ FragAt at(unsigned base) const {
         FragAt f = *this;
+        f.row += base; f.tr += base;
         asm volatile("" : "+v"(f.row), "+v"(f.tr));
         return f;
     }
-    // A / B fragment kk of row 32 t2 + (lane & 31): elements 16 kk + 8 h ..
-    __device__ __forceinline__ bf16x8 rows(const unsigned char* img, int t2, int kk) const {
-        return *(const bf16x8*)(img + (row ^ (kk << 5)) + 32 * t2 * DH * 2);
+    // A / B fragment kk of row 32 t2 + (lane & 31): elements 16 kk + 8 h ..;  img: bytes from the operand `base` names
+    __device__ __forceinline__ bf16x8 rows(const unsigned char* smem, int img, int t2, int kk) const {
+        return *(const bf16x8*)(smem + (row ^ (kk << 5)) + (img + 32 * t2 * DH * 2));
     }
     // transposed A fragment (tr_frag) of rows 32 t2 + 16 s + 4 h .., columns 32 di + (lane & 31)
-    __device__ __forceinline__ bf16x8 cols(const unsigned char* img, int t2, int s, int di) const {
-        const unsigned char* at = img + (32 * t2 + 16 * s) * DH * 2;
-        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(at + (tr ^ (di << 6))));
-        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(at + (tr ^ (di << 6) ^ 32) + 8 * DH * 2));
+    __device__ __forceinline__ bf16x8 cols(const unsigned char* smem, int img, int t2, int s, int di) const {
+        const int k = img + (32 * t2 + 16 * s) * DH * 2;
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(smem + (tr ^ (di << 6)) + k));
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(smem + (tr ^ ((di << 6) | 32)) + (k + 8 * DH * 2)));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
@@ -246,10 +250,50 @@ __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& r)
     return s * m.c;
 }
 
+// In the query-stationary kernels the distance bias without a cap rides the score product as one more step of 16: rows (the 32 a fragment covers) bring their
+// number in the tile, whole numbers up to 63 and so exact in bf16, columns bring their head's factor in three bf16 parts of 8
+// bits each; the products are exact and their sum is fp32.  x = q . k + f row, in raw score units, leaves to the
+// exponent's multiply-add a constant per lane and tile.  Right where |i - j| has one sign over the tile.
+struct BiasFrag {
+    unsigned row, f01, f2;               // 0 in the upper half of the wave, whose 8 elements of the step stay zero
+    __device__ __forceinline__ BiasFrag(float f, int lane) {
+        const __bf16 f0 = (__bf16)f, f1 = (__bf16)(f - (float)f0);
+        row = lane < 32 ? float_to_bf16((float)lane) : 0u;
+        f01 = lane < 32 ? pack_bf16x2(f, f - (float)f0) : 0u;
+        f2 = lane < 32 ? float_to_bf16(f - (float)f0 - (float)f1) : 0u;
+    }
+    // rows 32 t2 ..: every row of the fragment 32 t2 on
+    __device__ __forceinline__ floatx16 add(floatx16 S, int t2) const {
+        unsigned r = t2 == 0 ? row : float_to_bf16(bf16_to_float((unsigned short)row) + 32.f), zero = 0;   // (the upper half's 32 meets zeros)
+        asm volatile("" : "+v"(zero));   // formed here, not kept across the loop
+        const u32x4 x = {r | (r << 16), r, zero, zero}, y = {f01, f2, zero, zero};
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), S, 0, 0, 0);
+    }
+};
+
 // Masks shared by the kernels: how many keys at the front of a row every query sees (all of them without causality)
 __device__ __forceinline__ int seen_prefix(const AttendArgs& a, int b) {
     if (!a.causal) return a.T;
     return a.prefix != nullptr ? min(max(a.prefix[b], 0), a.T) : 0;
+}
+
+// Which of a half tile's 32 rows a lane's column sees, as bits (row n: bit n), applied to the registers with a bit-field
+// extract and a bitwise select: no lane masks in scalar registers, of which 16 comparisons would hold 32.
+__device__ __forceinline__ unsigned range_bits(int from, int past) {              // rows from <= n < past
+    const unsigned long long ones = 0xffffffffull;
+    const unsigned lo = (unsigned)(ones << min(max(from, 0), 32)), hi = (unsigned)(ones >> (32 - min(max(past, 0), 32)));
+    return lo & hi;
+}
+__device__ __forceinline__ unsigned doc_bits(const int* docs, int h, int mine) {  // rows acc_row(r, h) of the document `mine`; bit acc_row(r, 0)
+    unsigned m = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m |= docs[4 * h + acc_row(r, 0)] == mine ? 1u << acc_row(r, 0) : 0u;
+    return m;
+}
+__device__ __forceinline__ float pick(unsigned bits, int row, float x, float otherwise) {
+    const int k = (int)(bits << (31 - row)) >> 31;
+    const int xi = __builtin_bit_cast(int, x), oi = __builtin_bit_cast(int, otherwise);
+    return __builtin_bit_cast(float, (xi & k) | (oi & ~k));
 }
 
 // Pipeline of the three kernels: two stages of LDS, each a 64-row tile of both streamed operands.  A stage's loads go out when
@@ -282,6 +326,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
     const int qdoc = docs != nullptr ? docs[qc] : 0;
     const ScoreMap sm = score_map(a, CAP);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
+    const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
 
     TileWalk walk;
     walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
@@ -289,8 +334,8 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 
     int j = walk.next();
     if (j < walk.end) {
-        kdma.fetch(smem, j * TILE, wave);
-        vdma.fetch(smem + TB, j * TILE, wave);
+        kdma.fetch(smem, j, j == tiles - 1, wave);
+        vdma.fetch(smem + TB, j, j == tiles - 1, wave);
         if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
     }
     zero_unless<DH>(qdoc >= 0, qf);
@@ -313,21 +358,28 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         const bool go = walk.mine && jt <= wave_last, same = walk.whole, full = same && jt + TILE - 1 <= wave_least;
         j = walk.next();
         if (j < walk.end) {
-            kdma.fetch(smem + (stage ^ 1) * SB, j * TILE, wave);
-            vdma.fetch(smem + (stage ^ 1) * SB + TB, j * TILE, wave);
+            kdma.fetch(smem + (stage ^ 1) * SB, j, j == tiles - 1, wave);
+            vdma.fetch(smem + (stage ^ 1) * SB + TB, j, j == tiles - 1, wave);
             if (docs != nullptr && wave == 0) fetch_words(Kds[stage ^ 1], docs + j * TILE, T - j * TILE, lane);
         }
         if (!go) continue;                                          // wave-uniform
-        const FragAt<DH> fr = frags.fresh();
+        const FragAt<DH> fr = frags.at(stage * SB);
         floatx16 S[2];
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             zero16(S[t2]);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                S[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Ks, t2, kk), qf[kk], S[t2], 0, 0, 0);
+                S[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), qf[kk], S[t2], 0, 0, 0);
         }
-        if (CAP || BIAS) {
+        // y = c S + add, in base 2: the scale and what is the same for a lane's whole tile ride the exponent's multiply-add
+        float c = sm.c, add = 0.f;
+        if (BIAS && !CAP && (jt + TILE - 1 <= qw0 || pre <= qw0)) {  // wave-uniform: no visible key lies behind its query
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2) S[t2] = bf.add(S[t2], t2);
+            add = slope2 * (float)(jt - q);
+        } else if (CAP || BIAS) {
+            c = 1.f;
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
@@ -338,16 +390,13 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
                 }
         }
         if (!full) {                                                // wave-uniform
-            const int to = lim - jt - 4 * h;                        // row acc_row(r, 0) of the tile is seen iff <= to (and of the document)
-            const int* kd4 = Kd + 4 * h;
 #pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
+            for (int t2 = 0; t2 < 2; ++t2) {
+                unsigned bits = range_bits(0, lim + 1 - jt - 32 * t2 - 4 * h);
+                if (!same) bits &= doc_bits(Kd + 32 * t2, h, qdoc);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = 32 * t2 + acc_row(r, 0);
-                    const bool see = row <= to && (same || kd4[row] == qdoc);
-                    S[t2][r] = see ? S[t2][r] : MASKED;
-                }
+                for (int r = 0; r < 16; ++r) S[t2][r] = pick(bits, acc_row(r, 0), S[t2][r], MASKED);
+            }
         }
         float mx = NEG_BIG;
 #pragma unroll
@@ -355,15 +404,14 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[t2][r]);
         mx = xhalf_max(mx);
-        const float c = (CAP || BIAS) ? 1.f : sm.c;                 // the scale rides the exponent's multiply-add where nothing else used it
-        const float mn = fmaxf(m, mx * c);
+        const float mn = fmaxf(m, BIAS && !CAP ? fmaf(mx, c, add) : CAP ? mx : mx * c);
         const bool grew = mn > m;
         float rsum = 0.f;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = fast_exp2((CAP || BIAS) ? S[t2][r] - mn : fmaf(S[t2][r], c, -mn));
+                const float p = fast_exp2(CAP ? S[t2][r] - mn : fmaf(S[t2][r], c, add - mn));
                 S[t2][r] = p;
                 rsum += p;
             }
@@ -385,7 +433,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
                 const bf16x8 pb = pack_regs(S[t2], s);
 #pragma unroll
                 for (int di = 0; di < DI; ++di)
-                    O[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Vs, t2, s, di), pb,
+                    O[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, TB, t2, s, di), pb,
                                                                     O[di], 0, 0, 0);
             }
     }
@@ -438,6 +486,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const int qdoc = docs != nullptr ? docs[qc] : 0;
     const ScoreMap sm = score_map(a, CAP);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
+    const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
     const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
 
     TileWalk walk;
@@ -445,8 +494,8 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
     int j = walk.next();
     if (j < walk.end) {
-        kdma.fetch(smem, j * TILE, wave);
-        vdma.fetch(smem + TB, j * TILE, wave);
+        kdma.fetch(smem, j, j == tiles - 1, wave);
+        vdma.fetch(smem + TB, j, j == tiles - 1, wave);
         if (docs != nullptr && wave == 0) fetch_words(Kds[0], docs + j * TILE, T - j * TILE, lane);
     }
 
@@ -468,7 +517,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
         for (int r = 0; r < 16; ++r) del = acc_row(r, h) == ql ? dd[r] : del;
         del = xhalf_sum(del);                                       // one half holds the diagonal element, the other zero
     }
-    if (h == 0 && q < T) stats[((long)b * a.Hq + head) * T + q] = make_float2(lse_q, del);
+    if (h == 0 && q < T) stats[((long)b * a.Hq + head) * T + q] = make_float2(BIAS ? fmaf(slope2, (float)(q % TILE), lse_q) : lse_q, del);
 
     floatx16 dQt[DI];
 #pragma unroll
@@ -488,8 +537,8 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
         const bool go = walk.mine && jt <= wave_last, same = walk.whole;
         j = walk.next();
         if (j < walk.end) {
-            kdma.fetch(smem + (stage ^ 1) * SB, j * TILE, wave);
-            vdma.fetch(smem + (stage ^ 1) * SB + TB, j * TILE, wave);
+            kdma.fetch(smem + (stage ^ 1) * SB, j, j == tiles - 1, wave);
+            vdma.fetch(smem + (stage ^ 1) * SB + TB, j, j == tiles - 1, wave);
             if (docs != nullptr && wave == 0) fetch_words(Kds[stage ^ 1], docs + j * TILE, T - j * TILE, lane);
         }
         if (!go) continue;
@@ -498,49 +547,52 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
             const int kt0 = jt + 32 * t2;
             if (kt0 > wave_last) continue;                          // wave-uniform
             const bool full = same && kt0 + 31 <= wave_least;
-            const FragAt<DH> fr = frags.fresh();
+            const FragAt<DH> fr = frags.at(stage * SB);
             floatx16 S, dP;
             zero16(S); zero16(dP);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Ks, t2, kk), qf[kk], S, 0, 0, 0);
-                dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Vs, t2, kk), dof[kk], dP, 0, 0, 0);
+                S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), qf[kk], S, 0, 0, 0);
+                dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, t2, kk), dof[kk], dP, 0, 0, 0);
+            }
+            float c = sm.c, add = -lse_q;
+            if (BIAS && !CAP && (kt0 + 31 <= qw0 || pre <= qw0)) {  // as in the forward
+                S = bf.add(S, 0);
+                add += slope2 * (float)(kt0 - q);
+            } else if (BIAS && !CAP) {
+                c = 1.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    S[r] = fmaf(S[r], sm.c, -slope2 * fabsf((float)(q - kt0 - 4 * h) - (float)acc_row(r, 0)));
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float rr = 0.f, e;
-                if (CAP || BIAS) {
-                    e = map_score<CAP>(sm, S[r], rr);
+                if (CAP) {
+                    float rr;
+                    float e = map_score<CAP>(sm, S[r], rr);
                     if (BIAS) e = fmaf(-slope2, fabsf((float)(q - kt0 - 4 * h) - (float)acc_row(r, 0)), e);
-                    e -= lse_q;
+                    S[r] = fast_exp2(e - lse_q) * (dP[r] - del) * fmaf(-rr, rr, rr);      // (1 - tanh^2) / 4; the rest behind the product
                 } else {
-                    e = fmaf(S[r], sm.c, -lse_q);
+                    S[r] = fast_exp2(fmaf(S[r], c, add)) * (dP[r] - del);
                 }
-                float ds = fast_exp2(e) * a.scale * (dP[r] - del);
-                if (CAP) ds *= 4.f * rr * (1.f - rr);
-                S[r] = ds;
             }
             if (!full) {
-                const int to = lim - kt0 - 4 * h;
-                const int* kd4 = Kd + 32 * t2 + 4 * h;
+                unsigned bits = range_bits(0, lim + 1 - kt0 - 4 * h);
+                if (!same) bits &= doc_bits(Kd + 32 * t2, h, qdoc);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = acc_row(r, 0);
-                    const bool see = row <= to && (same || kd4[row] == qdoc);
-                    S[r] = see ? S[r] : 0.f;
-                }
+                for (int r = 0; r < 16; ++r) S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 dsb = pack_regs(S, s);
 #pragma unroll
                 for (int di = 0; di < DI; ++di)
-                    dQt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Ks, t2, s, di), dsb,
+                    dQt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, t2, s, di), dsb,
                                                                       dQt[di], 0, 0, 0);
             }
         }
     }
-    if (q < T) store_cols<DH>(dq + orow, dQt, qdoc >= 0 ? 1.f : 0.f, h, a.D);
+    if (q < T) store_cols<DH>(dq + orow, dQt, qdoc >= 0 ? (CAP ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
 }
 
 // ------------------------------------------------------------------------------ dK / dV (key-stationary, no atomics)
@@ -591,8 +643,8 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
         int j = walk.next();
 #define DPA_FETCH_Q(S_)                                                                                                  \
     if (j < walk.end) {                                                                                                  \
-        qdma.fetch(smem + (S_) * SB, j * TILE, wave);                                                                    \
-        odma.fetch(smem + (S_) * SB + TB, j * TILE, wave);                                                               \
+        qdma.fetch(smem + (S_) * SB, j, j == tiles - 1, wave);                                                                    \
+        odma.fetch(smem + (S_) * SB + TB, j, j == tiles - 1, wave);                                                               \
         if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2L * (T - j * TILE - 32 * wave), lane);  \
         else if (wave == 2 && docs != nullptr) fetch_words(Qds[S_], docs + j * TILE, T - j * TILE, lane);                \
     }
@@ -620,41 +672,42 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
                 const int qt0 = jt + 32 * t2;
                 if (qt0 + 31 < kw0 && kw0 >= pre) continue;         // wave-uniform
                 const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre) && qt0 + 32 <= T;
-                const FragAt<DH> fr = frags.fresh();
+                const FragAt<DH> fr = frags.at(stage * SB);
                 floatx16 S, dP;
                 zero16(S); zero16(dP);
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
-                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Qs, t2, kk), kf[kk], S, 0, 0, 0);
-                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(Os, t2, kk), vf[kk], dP, 0, 0, 0);
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), kf[kk], S, 0, 0, 0);
+                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, t2, kk), vf[kk], dP, 0, 0, 0);
                 }
                 const float2* ld4 = lds_s + 32 * t2 + 4 * h;
+                // BIAS: ld.x holds lse + slope (i mod 64), so that -slope (i - j) - lse = slope (j - jt) - ld.x where no query
+                // that sees a key lies in front of it, and elsewhere the sign is put right per element
+                const bool linear = qt0 >= kw0 + 31 || pre <= qt0;
+                const float add = slope2 * (float)(key - jt);
+                const float behind = !BIAS || linear ? 0.f : 2.f * slope2;
+                if (BIAS && !CAP && !linear) {                      // in raw units, in front of the scale
+                    const float f = behind / sm.c;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) S[r] = fmaf(-f, fmaxf((float)(key - qt0 - 4 * h) - (float)acc_row(r, 0), 0.f), S[r]);
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int row = acc_row(r, 0);
-                    float rr = 0.f, e;
-                    if (CAP || BIAS) {
-                        e = map_score<CAP>(sm, S[r], rr);
-                        if (BIAS) e = fmaf(-slope2, fabsf((float)(qt0 + 4 * h - key) + (float)row), e);
-                        e -= ld4[row].x;
-                    } else {
-                        e = fmaf(S[r], sm.c, -ld4[row].x);
-                    }
-                    const float p = fast_exp2(e);
-                    float ds = p * a.scale * (dP[r] - ld4[row].y);
-                    if (CAP) ds *= 4.f * rr * (1.f - rr);
-                    S[r] = p;
-                    dP[r] = ds;
+                    const float2 ld = ld4[row];
+                    float rr, off = BIAS ? ld.x - add : ld.x;
+                    if (BIAS && CAP) off = fmaf(behind, fmaxf((float)(key - qt0 - 4 * h) - (float)row, 0.f), off);
+                    S[r] = fast_exp2(CAP ? map_score<true>(sm, S[r], rr) - off : fmaf(S[r], sm.c, -off));
+                    dP[r] = S[r] * (dP[r] - ld.y);
+                    if (CAP) dP[r] *= fmaf(-rr, rr, rr);            // (1 - tanh^2) / 4; the rest behind the product
                 }
                 if (!full) {
-                    const int from = key_from - qt0 - 4 * h, past = T - qt0 - 4 * h;   // row acc_row(r, 0) sees this lane's key iff from <= row < past
-                    const int* qd4 = Qd + 32 * t2 + 4 * h;
+                    unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
+                    if (!same) bits &= doc_bits(Qd + 32 * t2, h, kdoc);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int row = acc_row(r, 0);
-                        const bool see = row >= from && row < past && (same || qd4[row] == kdoc);
-                        S[r] = see ? S[r] : 0.f;
-                        dP[r] = see ? dP[r] : 0.f;
+                        S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
+                        dP[r] = pick(bits, acc_row(r, 0), dP[r], 0.f);
                     }
                 }
 #pragma unroll
@@ -662,14 +715,15 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
                     const bf16x8 pb = pack_regs(S, s), dsb = pack_regs(dP, s);
 #pragma unroll
                     for (int di = 0; di < DI; ++di) {
-                        dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Os, t2, s, di), pb, dVt[di], 0, 0, 0);
-                        dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(Qs, t2, s, di), dsb, dKt[di], 0, 0, 0);
+                        dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, TB, t2, s, di), pb, dVt[di], 0, 0, 0);
+                        dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, t2, s, di), dsb, dKt[di], 0, 0, 0);
                     }
                 }
             }
         }
 #undef DPA_FETCH_Q
     }
+    const float dscale = (CAP ? 4.f : 1.f) * a.scale;               // of dS: (1 - tanh^2) was left a quarter
     if (key < T && part != nullptr) {
         const long row = (((long)b * T + key) * a.Hkv + hk) * a.D, n = (long)a.B * T * a.Hkv * a.D;
         float* to = part + (long)(hq0 / heads % (a.Hq / a.Hkv / heads)) * 2 * n + row;
@@ -679,13 +733,13 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * di + 8 * g + 4 * h;
                 if (d < a.D) {
-                    *(float4*)(to + d) = make_float4(dKt[di][4 * g], dKt[di][4 * g + 1], dKt[di][4 * g + 2], dKt[di][4 * g + 3]);
+                    *(float4*)(to + d) = make_float4(dKt[di][4 * g] * dscale, dKt[di][4 * g + 1] * dscale, dKt[di][4 * g + 2] * dscale, dKt[di][4 * g + 3] * dscale);
                     *(float4*)(to + n + d) = make_float4(dVt[di][4 * g], dVt[di][4 * g + 1], dVt[di][4 * g + 2], dVt[di][4 * g + 3]);
                 }
             }
     } else if (key < T) {
         const long row = (((long)b * T + key) * a.Hkv + hk) * a.D;
-        store_cols<DH>(dk + row, dKt, kdoc >= 0 ? 1.f : 0.f, h, a.D);
+        store_cols<DH>(dk + row, dKt, kdoc >= 0 ? dscale : 0.f, h, a.D);
         store_cols<DH>(dv + row, dVt, kdoc >= 0 ? 1.f : 0.f, h, a.D);
     }
 }
