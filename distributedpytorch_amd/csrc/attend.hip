@@ -56,17 +56,19 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const int* __restrict__
 }
 
 // Walks the 64-row tiles first .. end - 1 that a workgroup's rows can share a document with.  `mine` / `whole`: whether the
-// wave's own 32 rows meet the current tile, and whether every pair of the two is of one document.
+// wave's own 32 rows meet the current tile, and whether every pair of the two is of one document.  Up or down: workgroups
+// of a head that run at once should read the same tiles at once, so that they find them in their XCD's L2; queries (whose
+// last tile differs) start at the front together, keys (whose first differs) at the end.
+template <bool DOWN>
 struct TileWalk {
     const int4* rg;                      // nullptr: no documents, every tile is visited whole
-    int base, end, j;
+    int base, first, end;                // base: tiles behind us, in walking order
     DocRange block, wave;
     unsigned long long todo, mine_bits, whole_bits, pad_bits;
     bool mine, whole, pad;                // pad: some of the tile's rows are padding
 
     __device__ __forceinline__ void look(const int4& v) {          // v: this lane's entry (of a tile in range)
-        const int lane = threadIdx.x & 63, t = base + lane;
-        bool a = t < end, b = true, c = true, p = false;
+        bool a = base + (int)(threadIdx.x & 63) < end - first, b = true, c = true, p = false;
         if (rg != nullptr) {
             const DocRange d = merge(DocRange{v.x, v.y}, DocRange{v.z, v.w});
             a = a && meets(d, block);
@@ -76,14 +78,14 @@ struct TileWalk {
         }
         todo = __ballot(a); mine_bits = __ballot(b); whole_bits = __ballot(c); pad_bits = __ballot(p);
     }
+    __device__ __forceinline__ int tile(int n) const { return DOWN ? end - 1 - n : first + n; }
     __device__ __forceinline__ int4 entry() const {
-        const int t = base + (int)(threadIdx.x & 63);
-        return rg != nullptr ? rg[min(t, end - 1)] : make_int4(0, 0, 0, 0);
+        return rg != nullptr ? rg[tile(min(base + (int)(threadIdx.x & 63), end - first - 1))] : make_int4(0, 0, 0, 0);
     }
-    // Rows row0 .. row0 + 127 (a multiple of 128; the wave's own are 32 w ..) against tiles first .. end_ - 1, end_ > first.  One
+    // Rows row0 .. row0 + 127 (a multiple of 128; the wave's own are 32 w ..) against tiles first_ .. end_ - 1, end_ > first_.  One
     // round of loads: the entries of the rows' own two tiles and the first 64 of the walk go out together.
-    __device__ __forceinline__ void open(const int4* rg_, int tiles, int row0, int w, int first, int end_) {
-        rg = rg_; base = first; end = end_;
+    __device__ __forceinline__ void open(const int4* rg_, int tiles, int row0, int w, int first_, int end_) {
+        rg = rg_; base = 0; first = first_; end = end_;
         int4 v = entry();
         if (rg != nullptr) {
             const int t0 = row0 / TILE;
@@ -98,18 +100,18 @@ struct TileWalk {
         }
         look(v);
     }
-    __device__ __forceinline__ void restart(int first) { base = first; look(entry()); }
+    __device__ __forceinline__ void restart() { base = 0; look(entry()); }
     // the next tile, or `end` when there is none
     __device__ __forceinline__ int next() {
         while (todo == 0) {
             base += 64;
-            if (base >= end) { base = end; return end; }
+            if (base >= end - first) { base = end - first; return end; }
             look(entry());
         }
         const int bit = __ffsll((long long)todo) - 1;
         todo &= todo - 1;
         mine = (mine_bits >> bit) & 1; whole = (whole_bits >> bit) & 1; pad = (pad_bits >> bit) & 1;
-        return base + bit;
+        return tile(base + bit);
     }
 };
 
@@ -220,10 +222,10 @@ __device__ __forceinline__ void zero_unless(bool live, bf16x8 (&f)[DH / 16]) {
     }
 }
 
-template <int DH>
-__device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, const floatx16 (&acc)[DH / 32], float scale, int h, int D) {
+template <int DI>
+__device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, const floatx16 (&acc)[DI], float scale, int h, int D) {
 #pragma unroll
-    for (int di = 0; di < DH / 32; ++di)
+    for (int di = 0; di < DI; ++di)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = 32 * di + 8 * g + 4 * h;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
     const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
 
-    TileWalk walk;
+    TileWalk<false> walk;
     walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
 
@@ -447,13 +449,13 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         for (int di = 0; di < DI; ++di)
 #pragma unroll
             for (int r = 0; r < 16; ++r) O[di][r] *= inv;
-        store_cols<DH>(out + row, O, 1.f, h, a.D);
+        store_cols(out + row, O, 1.f, h, a.D);
         if (rest != nullptr) {
 #pragma unroll
             for (int di = 0; di < DI; ++di)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) O[di][r] -= bf16_to_float(float_to_bf16(O[di][r]));
-            store_cols<DH>(rest + row, O, 1.f, h, a.D);
+            store_cols(rest + row, O, 1.f, h, a.D);
         }
         if (h == 0) lse2[((long)b * a.Hq + head) * T + q] = empty ? 1.0e30f : m + __log2f(l);
     }
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
     const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
 
-    TileWalk walk;
+    TileWalk<false> walk;
     walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
     const int wave_last = max(min(qw0 + 31, T - 1), pre - 1), wave_least = max(min(qw0, T - 1), pre - 1);
     int j = walk.next();
@@ -592,25 +594,80 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
             }
         }
     }
-    if (q < T) store_cols<DH>(dq + orow, dQt, qdoc >= 0 ? (CAP ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
+    if (q < T) store_cols(dq + orow, dQt, qdoc >= 0 ? (CAP ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
 }
 
 // ------------------------------------------------------------------------------ dK / dV (key-stationary, no atomics)
 // A key head's gradient sums over its group of query heads.  Where that leaves few workgroups (kv_parts below) the group is
 // cut: a workgroup takes `heads` of its query heads and writes its sums in fp32 to part [part][B, T, Hkv, D], dK and then dV,
 // and fold_parts_kernel adds the parts in order.
-template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
-                                                               const float2* __restrict__ stats, unsigned short* __restrict__ dk,
-                                                               unsigned short* __restrict__ dv, float* __restrict__ part, int heads) {
-    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+// P and dS / scale (a quarter of it under a cap) of 32 queries (registers) and this lane's key, in place of S and dP.
+// ld: the queries' (lse, delta) from row 4 h on; BIAS: lse + slope (i mod 64), so that -slope (i - j) - lse =
+// slope (j - jt) - ld.x where no query that sees a key lies in front of it (`linear`), and elsewhere the sign is put right
+// per element.  to_key: key - first query - 4 h; in_tile: key - first query of the 64-row tile.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void key_side(floatx16& S, floatx16& dP, const float2* ld, const ScoreMap& sm, float slope2, bool linear, int to_key, int in_tile) {
+    const float add = slope2 * (float)in_tile, behind = !BIAS || linear ? 0.f : 2.f * slope2;
+    if (BIAS && !CAP && !linear) {                                  // in raw units, in front of the scale
+        const float f = behind / sm.c;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[r] = fmaf(-f, fmaxf((float)to_key - (float)acc_row(r, 0), 0.f), S[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = acc_row(r, 0);
+        const float2 x = ld[row];
+        float rr, off = BIAS ? x.x - add : x.x;
+        if (BIAS && CAP) off = fmaf(behind, fmaxf((float)to_key - (float)row, 0.f), off);
+        S[r] = fast_exp2(CAP ? map_score<true>(sm, S[r], rr) - off : fmaf(S[r], sm.c, -off));
+        dP[r] = S[r] * (dP[r] - x.y);
+        if (CAP) dP[r] *= fmaf(-rr, rr, rr);                        // (1 - tanh^2) / 4; the rest behind the product
+    }
+}
+
+// this lane's key's channels d0 .. d0 + 32 DI - 1: rounded to dk / dv, or in fp32 to the workgroup's part (KvOut below)
+struct KvOut {
+    unsigned short *dk, *dv;
+    float* part;                         // nullptr: whole groups
+    int heads;                           // query heads of a workgroup
+};
+template <bool CAP, int DI>
+__device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, const floatx16 (&dKt)[DI], const floatx16 (&dVt)[DI], int b, int key, int hq0,
+                                          bool live, int d0, int h) {
+    if (key >= a.T) return;
+    const int group = a.Hq / a.Hkv;
+    const long row = (((long)b * a.T + key) * a.Hkv + hq0 / group) * a.D + d0;
+    const float kscale = live ? (CAP ? 4.f : 1.f) * a.scale : 0.f, vscale = live ? 1.f : 0.f;
+    if (o.part == nullptr) {
+        store_cols(o.dk + row, dKt, kscale, h, a.D - d0);
+        store_cols(o.dv + row, dVt, vscale, h, a.D - d0);
+        return;
+    }
+    const long n = (long)a.B * a.T * a.Hkv * a.D;
+    float* to = o.part + (long)(hq0 % group / o.heads) * 2 * n + row;
+#pragma unroll
+    for (int di = 0; di < DI; ++di)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * di + 8 * g + 4 * h;
+            if (d0 + d < a.D) {
+                *(float4*)(to + d) = make_float4(dKt[di][4 * g] * kscale, dKt[di][4 * g + 1] * kscale, dKt[di][4 * g + 2] * kscale, dKt[di][4 * g + 3] * kscale);
+                *(float4*)(to + n + d) = make_float4(dVt[di][4 * g] * vscale, dVt[di][4 * g + 1] * vscale, dVt[di][4 * g + 2] * vscale, dVt[di][4 * g + 3] * vscale);
+            }
+        }
+}
+
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+                                                               const float2* __restrict__ stats, KvOut o) {
+    constexpr int DH = 64, KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
     __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
     __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kl = lane & 31, h = lane >> 5;
     const FragAt<DH> frags(lane);
-    const int hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
+    const int heads = o.heads, hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
     const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * wave, key = kw0 + kl, keyc = min(key, T - 1);
     const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
     const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
@@ -630,7 +687,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
     for (int di = 0; di < DI; ++di) { zero16(dKt[di]); zero16(dVt[di]); }
 
     const int first = k0 < pre ? 0 : k0 / TILE;                     // in front of the first key only a prefix key is seen
-    TileWalk walk;
+    TileWalk<true> walk;
     walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, k0, wave, first, tiles);
     const int key_from = key < pre ? -(1 << 30) : key;              // the first query that sees this lane's key
 
@@ -639,7 +696,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
         const TileDma<DH> odma(dout + ((long)b * T * a.Hq + head) * a.D, (long)a.Hq * a.D, T, a.D, tid);
         const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
         const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-        if (head > hq0) walk.restart(first);
+        if (head > hq0) walk.restart();
         int j = walk.next();
 #define DPA_FETCH_Q(S_)                                                                                                  \
     if (j < walk.end) {                                                                                                  \
@@ -681,26 +738,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
                     dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, t2, kk), vf[kk], dP, 0, 0, 0);
                 }
                 const float2* ld4 = lds_s + 32 * t2 + 4 * h;
-                // BIAS: ld.x holds lse + slope (i mod 64), so that -slope (i - j) - lse = slope (j - jt) - ld.x where no query
-                // that sees a key lies in front of it, and elsewhere the sign is put right per element
-                const bool linear = qt0 >= kw0 + 31 || pre <= qt0;
-                const float add = slope2 * (float)(key - jt);
-                const float behind = !BIAS || linear ? 0.f : 2.f * slope2;
-                if (BIAS && !CAP && !linear) {                      // in raw units, in front of the scale
-                    const float f = behind / sm.c;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) S[r] = fmaf(-f, fmaxf((float)(key - qt0 - 4 * h) - (float)acc_row(r, 0), 0.f), S[r]);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = acc_row(r, 0);
-                    const float2 ld = ld4[row];
-                    float rr, off = BIAS ? ld.x - add : ld.x;
-                    if (BIAS && CAP) off = fmaf(behind, fmaxf((float)(key - qt0 - 4 * h) - (float)row, 0.f), off);
-                    S[r] = fast_exp2(CAP ? map_score<true>(sm, S[r], rr) - off : fmaf(S[r], sm.c, -off));
-                    dP[r] = S[r] * (dP[r] - ld.y);
-                    if (CAP) dP[r] *= fmaf(-rr, rr, rr);            // (1 - tanh^2) / 4; the rest behind the product
-                }
+                key_side<CAP, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
                 if (!full) {
                     unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
                     if (!same) bits &= doc_bits(Qd + 32 * t2, h, kdoc);
@@ -723,25 +761,134 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attend_bwd_kv_kernel(At
         }
 #undef DPA_FETCH_Q
     }
-    const float dscale = (CAP ? 4.f : 1.f) * a.scale;               // of dS: (1 - tanh^2) was left a quarter
-    if (key < T && part != nullptr) {
-        const long row = (((long)b * T + key) * a.Hkv + hk) * a.D, n = (long)a.B * T * a.Hkv * a.D;
-        float* to = part + (long)(hq0 / heads % (a.Hq / a.Hkv / heads)) * 2 * n + row;
+    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, 0, h);
+}
+
+// The same at width 128, where one wave cannot hold a key block: two accumulators of 32 keys x 128 channels and the two
+// stationary operands are 192 registers, and with what is left every fragment read waits for itself (WIDE_FIGURES).  Two
+// waves share 32 keys instead.  Each forms P and dS of one half of the tile's queries against all channels and accumulates
+// one half of the channels over all queries; the halves' P and dS, rounded as the products want them anyway, change hands
+// through LDS (4 KiB a wave), the own half's products running in front of the barrier that this takes.
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(512, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+                                                               const float2* __restrict__ stats, KvOut o) {
+    constexpr int DH = 128, KK = DH / 16, DI = DH / 64, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
+    __shared__ u32x4 swap[8][4][64];
+    __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
+    __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kl = lane & 31, h = lane >> 5;
+    const FragAt<DH> frags(lane);
+    FragAt<DH> outs = frags;                                        // at my half of the channels
+    outs.tr ^= (wave & 1) << 7;
+    const int mine = wave & 1, lo = wave >> 2;                      // my half of the queries and of the output's channels; which operand's tile I load
+    const int heads = o.heads, hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
+    const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * (wave >> 1), key = kw0 + kl, keyc = min(key, T - 1);
+    const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
+    const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
+    const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
+    const int tiles = (T + TILE - 1) / TILE;
+    const int pre = seen_prefix(a, b);
+    const int kdoc = docs != nullptr ? docs[keyc] : 0;
+    const ScoreMap sm = score_map(a, CAP);
+
+    bf16x8 kf[KK], vf[KK];
+    load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kf);
+    load_frags<DH>(vbase + (long)keyc * a.vt, h, a.D, vf);
+    zero_unless<DH>(kdoc >= 0, kf);
+    zero_unless<DH>(kdoc >= 0, vf);
+    floatx16 dKt[DI], dVt[DI];
 #pragma unroll
-        for (int di = 0; di < DI; ++di)
+    for (int di = 0; di < DI; ++di) { zero16(dKt[di]); zero16(dVt[di]); }
+
+    const int first = k0 < pre ? 0 : k0 / TILE;                     // in front of the first key only a prefix key is seen
+    TileWalk<true> walk;
+    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, k0, wave >> 1, first, tiles);
+    const int key_from = key < pre ? -(1 << 30) : key;              // the first query that sees this lane's key
+
+    // dV^T += dO^T P, dK^T += Q^T dS over 32 queries and my 64 channels; fr: at those queries' rows
+    const auto add_outputs = [&](const FragAt<DH>& fr, const u32x4 (&x)[4]) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = 32 * di + 8 * g + 4 * h;
-                if (d < a.D) {
-                    *(float4*)(to + d) = make_float4(dKt[di][4 * g] * dscale, dKt[di][4 * g + 1] * dscale, dKt[di][4 * g + 2] * dscale, dKt[di][4 * g + 3] * dscale);
-                    *(float4*)(to + n + d) = make_float4(dVt[di][4 * g], dVt[di][4 * g + 1], dVt[di][4 * g + 2], dVt[di][4 * g + 3]);
-                }
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int di = 0; di < DI; ++di) {
+                dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, TB, 0, s, di), __builtin_bit_cast(bf16x8, x[s]), dVt[di], 0, 0, 0);
+                dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, 0, s, di), __builtin_bit_cast(bf16x8, x[2 + s]), dKt[di], 0, 0, 0);
             }
-    } else if (key < T) {
-        const long row = (((long)b * T + key) * a.Hkv + hk) * a.D;
-        store_cols<DH>(dk + row, dKt, kdoc >= 0 ? dscale : 0.f, h, a.D);
-        store_cols<DH>(dv + row, dVt, kdoc >= 0 ? 1.f : 0.f, h, a.D);
+    };
+    for (int head = hq0; head < hq0 + heads; ++head) {
+        const unsigned short* from = lo == 0 ? (const unsigned short*)a.q + b * a.qb + head * a.qh : dout + ((long)b * T * a.Hq + head) * a.D;
+        const TileDma<DH> dma(from, lo == 0 ? a.qt : (long)a.Hq * a.D, T, a.D, tid & 255);
+        const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
+        const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
+        if (head > hq0) walk.restart();
+        int j = walk.next();
+#define DPA_FETCH_Q(S_)                                                                                                  \
+    if (j < walk.end) {                                                                                                  \
+        dma.fetch(smem + (S_) * SB + lo * TB, j, j == tiles - 1, wave & 3);                                              \
+        if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2L * (T - j * TILE - 32 * wave), lane);  \
+        else if (wave == 2 && docs != nullptr) fetch_words(Qds[S_], docs + j * TILE, T - j * TILE, lane);                \
     }
+        __syncthreads();                                            // the stages are free of the head before
+        DPA_FETCH_Q(0)
+        for (int stage = 0; j < walk.end; stage ^= 1) {
+            const float2* lds_s = lds_ss[stage];
+            const int* Qd = Qds[stage];
+            tiles_landed();
+            __syncthreads();
+            if (walk.pad) {
+                clear_padding<DH>(smem + stage * SB + lo * TB, Qd, tid & 255);
+                __syncthreads();
+            }
+            const int jt = j * TILE;
+            const bool go = walk.mine && (jt + TILE - 1 >= kw0 || kw0 < pre), same = walk.whole;
+            const bool live0 = go && (jt + 31 >= kw0 || kw0 < pre);  // the front half's queries see some of my keys (the back half's do if go)
+            j = walk.next();
+            DPA_FETCH_Q(stage ^ 1)
+            u32x4 own[4];
+            if (mine ? go : live0) {                                // wave-uniform
+                const int qt0 = jt + 32 * mine;
+                const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre) && qt0 + 32 <= T;
+                const FragAt<DH> fr = frags.at(stage * SB + mine * 32 * DH * 2);
+                floatx16 S, dP;
+                zero16(S); zero16(dP);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, 0, kk), kf[kk], S, 0, 0, 0);
+                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, 0, kk), vf[kk], dP, 0, 0, 0);
+                }
+                // rows = queries (registers), column = this lane's key
+                const float2* ld4 = lds_s + 32 * mine + 4 * h;
+                key_side<CAP, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
+                if (!full) {
+                    unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
+                    if (!same) bits &= doc_bits(Qd + 32 * mine, h, kdoc);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
+                        dP[r] = pick(bits, acc_row(r, 0), dP[r], 0.f);
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    own[s] = __builtin_bit_cast(u32x4, pack_regs(S, s));
+                    own[2 + s] = __builtin_bit_cast(u32x4, pack_regs(dP, s));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) swap[wave][i][lane] = own[i];
+                add_outputs(outs.at(stage * SB + mine * 32 * DH * 2), own);
+            }
+            __syncthreads();                                        // the other half's P and dS are there
+            if (mine ? live0 : go) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) own[i] = swap[wave ^ 1][i][lane];
+                add_outputs(outs.at(stage * SB + (1 - mine) * 32 * DH * 2), own);
+            }
+        }
+#undef DPA_FETCH_Q
+    }
+    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, 64 * mine, h);
 }
 
 // dk, dv [n] = the sum of their parts [parts][2][n] in order, rounded once (n a multiple of 8)
@@ -770,8 +917,11 @@ void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* 
     hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
                        (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
     const int parts = part != nullptr ? attend_kv_parts(a) : 1, heads = a.Hq / a.Hkv / parts;
-    hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout,
-                       (const float2*)stats, (unsigned short*)dk, (unsigned short*)dv, part, heads);
+    const KvOut o{(unsigned short*)dk, (unsigned short*)dv, part, heads};
+    if constexpr (DH == 64)
+        hipLaunchKernelGGL((attend_bwd_kv_kernel<CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
+    else
+        hipLaunchKernelGGL((attend_bwd_kv_wide_kernel<CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(512), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
     if (part != nullptr) {
         const long n = (long)a.B * a.T * a.Hkv * a.D, grid = (2 * n / 8 + 255) / 256;
         hipLaunchKernelGGL(fold_parts_kernel, dim3((unsigned)(grid > 8192 ? 8192 : grid)), dim3(256), 0, st, part, parts, n, (unsigned short*)dk, (unsigned short*)dv);
