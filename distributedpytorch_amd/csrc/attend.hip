@@ -625,7 +625,7 @@ __device__ __forceinline__ void key_side(floatx16& S, floatx16& dP, const float2
     }
 }
 
-// this lane's key's channels d0 .. d0 + 32 DI - 1: rounded to dk / dv, or in fp32 to the workgroup's part (KvOut below)
+// this lane's key: rounded to dk / dv, or in fp32 to the workgroup's part (KvOut below)
 struct KvOut {
     unsigned short *dk, *dv;
     float* part;                         // nullptr: whole groups
@@ -633,14 +633,14 @@ struct KvOut {
 };
 template <bool CAP, int DI>
 __device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, const floatx16 (&dKt)[DI], const floatx16 (&dVt)[DI], int b, int key, int hq0,
-                                          bool live, int d0, int h) {
+                                          bool live, int h) {
     if (key >= a.T) return;
     const int group = a.Hq / a.Hkv;
-    const long row = (((long)b * a.T + key) * a.Hkv + hq0 / group) * a.D + d0;
+    const long row = (((long)b * a.T + key) * a.Hkv + hq0 / group) * a.D;
     const float kscale = live ? (CAP ? 4.f : 1.f) * a.scale : 0.f, vscale = live ? 1.f : 0.f;
     if (o.part == nullptr) {
-        store_cols(o.dk + row, dKt, kscale, h, a.D - d0);
-        store_cols(o.dv + row, dVt, vscale, h, a.D - d0);
+        store_cols(o.dk + row, dKt, kscale, h, a.D);
+        store_cols(o.dv + row, dVt, vscale, h, a.D);
         return;
     }
     const long n = (long)a.B * a.T * a.Hkv * a.D;
@@ -650,17 +650,17 @@ __device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, c
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = 32 * di + 8 * g + 4 * h;
-            if (d0 + d < a.D) {
+            if (d < a.D) {
                 *(float4*)(to + d) = make_float4(dKt[di][4 * g] * kscale, dKt[di][4 * g + 1] * kscale, dKt[di][4 * g + 2] * kscale, dKt[di][4 * g + 3] * kscale);
                 *(float4*)(to + n + d) = make_float4(dVt[di][4 * g] * vscale, dVt[di][4 * g + 1] * vscale, dVt[di][4 * g + 2] * vscale, dVt[di][4 * g + 3] * vscale);
             }
         }
 }
 
-template <bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+template <int DH, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
                                                                const float2* __restrict__ stats, KvOut o) {
-    constexpr int DH = 64, KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
     __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
     __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
@@ -761,134 +761,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
         }
 #undef DPA_FETCH_Q
     }
-    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, 0, h);
-}
-
-// The same at width 128, where one wave cannot hold a key block: two accumulators of 32 keys x 128 channels and the two
-// stationary operands are 192 registers, and with what is left every fragment read waits for itself (WIDE_FIGURES).  Two
-// waves share 32 keys instead.  Each forms P and dS of one half of the tile's queries against all channels and accumulates
-// one half of the channels over all queries; the halves' P and dS, rounded as the products want them anyway, change hands
-// through LDS (4 KiB a wave), the own half's products running in front of the barrier that this takes.
-template <bool CAP, bool BIAS>
-__global__ __launch_bounds__(512, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
-                                                               const float2* __restrict__ stats, KvOut o) {
-    constexpr int DH = 128, KK = DH / 16, DI = DH / 64, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
-    __shared__ u32x4 swap[8][4][64];
-    __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
-    __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kl = lane & 31, h = lane >> 5;
-    const FragAt<DH> frags(lane);
-    FragAt<DH> outs = frags;                                        // at my half of the channels
-    outs.tr ^= (wave & 1) << 7;
-    const int mine = wave & 1, lo = wave >> 2;                      // my half of the queries and of the output's channels; which operand's tile I load
-    const int heads = o.heads, hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
-    const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * (wave >> 1), key = kw0 + kl, keyc = min(key, T - 1);
-    const unsigned short* kbase = (const unsigned short*)a.k + b * a.kb + hk * a.kh;
-    const unsigned short* vbase = (const unsigned short*)a.v + b * a.vb + hk * a.vh;
-    const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
-    const int tiles = (T + TILE - 1) / TILE;
-    const int pre = seen_prefix(a, b);
-    const int kdoc = docs != nullptr ? docs[keyc] : 0;
-    const ScoreMap sm = score_map(a, CAP);
-
-    bf16x8 kf[KK], vf[KK];
-    load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kf);
-    load_frags<DH>(vbase + (long)keyc * a.vt, h, a.D, vf);
-    zero_unless<DH>(kdoc >= 0, kf);
-    zero_unless<DH>(kdoc >= 0, vf);
-    floatx16 dKt[DI], dVt[DI];
-#pragma unroll
-    for (int di = 0; di < DI; ++di) { zero16(dKt[di]); zero16(dVt[di]); }
-
-    const int first = k0 < pre ? 0 : k0 / TILE;                     // in front of the first key only a prefix key is seen
-    TileWalk<true> walk;
-    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, k0, wave >> 1, first, tiles);
-    const int key_from = key < pre ? -(1 << 30) : key;              // the first query that sees this lane's key
-
-    // dV^T += dO^T P, dK^T += Q^T dS over 32 queries and my 64 channels; fr: at those queries' rows
-    const auto add_outputs = [&](const FragAt<DH>& fr, const u32x4 (&x)[4]) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int di = 0; di < DI; ++di) {
-                dVt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, TB, 0, s, di), __builtin_bit_cast(bf16x8, x[s]), dVt[di], 0, 0, 0);
-                dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, 0, s, di), __builtin_bit_cast(bf16x8, x[2 + s]), dKt[di], 0, 0, 0);
-            }
-    };
-    for (int head = hq0; head < hq0 + heads; ++head) {
-        const unsigned short* from = lo == 0 ? (const unsigned short*)a.q + b * a.qb + head * a.qh : dout + ((long)b * T * a.Hq + head) * a.D;
-        const TileDma<DH> dma(from, lo == 0 ? a.qt : (long)a.Hq * a.D, T, a.D, tid & 255);
-        const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
-        const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-        if (head > hq0) walk.restart();
-        int j = walk.next();
-#define DPA_FETCH_Q(S_)                                                                                                  \
-    if (j < walk.end) {                                                                                                  \
-        dma.fetch(smem + (S_) * SB + lo * TB, j, j == tiles - 1, wave & 3);                                              \
-        if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2L * (T - j * TILE - 32 * wave), lane);  \
-        else if (wave == 2 && docs != nullptr) fetch_words(Qds[S_], docs + j * TILE, T - j * TILE, lane);                \
-    }
-        __syncthreads();                                            // the stages are free of the head before
-        DPA_FETCH_Q(0)
-        for (int stage = 0; j < walk.end; stage ^= 1) {
-            const float2* lds_s = lds_ss[stage];
-            const int* Qd = Qds[stage];
-            tiles_landed();
-            __syncthreads();
-            if (walk.pad) {
-                clear_padding<DH>(smem + stage * SB + lo * TB, Qd, tid & 255);
-                __syncthreads();
-            }
-            const int jt = j * TILE;
-            const bool go = walk.mine && (jt + TILE - 1 >= kw0 || kw0 < pre), same = walk.whole;
-            const bool live0 = go && (jt + 31 >= kw0 || kw0 < pre);  // the front half's queries see some of my keys (the back half's do if go)
-            j = walk.next();
-            DPA_FETCH_Q(stage ^ 1)
-            u32x4 own[4];
-            if (mine ? go : live0) {                                // wave-uniform
-                const int qt0 = jt + 32 * mine;
-                const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre) && qt0 + 32 <= T;
-                const FragAt<DH> fr = frags.at(stage * SB + mine * 32 * DH * 2);
-                floatx16 S, dP;
-                zero16(S); zero16(dP);
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, 0, kk), kf[kk], S, 0, 0, 0);
-                    dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, 0, kk), vf[kk], dP, 0, 0, 0);
-                }
-                // rows = queries (registers), column = this lane's key
-                const float2* ld4 = lds_s + 32 * mine + 4 * h;
-                key_side<CAP, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
-                if (!full) {
-                    unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
-                    if (!same) bits &= doc_bits(Qd + 32 * mine, h, kdoc);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
-                        dP[r] = pick(bits, acc_row(r, 0), dP[r], 0.f);
-                    }
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    own[s] = __builtin_bit_cast(u32x4, pack_regs(S, s));
-                    own[2 + s] = __builtin_bit_cast(u32x4, pack_regs(dP, s));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) swap[wave][i][lane] = own[i];
-                add_outputs(outs.at(stage * SB + mine * 32 * DH * 2), own);
-            }
-            __syncthreads();                                        // the other half's P and dS are there
-            if (mine ? live0 : go) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) own[i] = swap[wave ^ 1][i][lane];
-                add_outputs(outs.at(stage * SB + (1 - mine) * 32 * DH * 2), own);
-            }
-        }
-#undef DPA_FETCH_Q
-    }
-    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, 64 * mine, h);
+    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
 }
 
 // dk, dv [n] = the sum of their parts [parts][2][n] in order, rounded once (n a multiple of 8)
@@ -918,10 +791,7 @@ void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* 
                        (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
     const int parts = part != nullptr ? attend_kv_parts(a) : 1, heads = a.Hq / a.Hkv / parts;
     const KvOut o{(unsigned short*)dk, (unsigned short*)dv, part, heads};
-    if constexpr (DH == 64)
-        hipLaunchKernelGGL((attend_bwd_kv_kernel<CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
-    else
-        hipLaunchKernelGGL((attend_bwd_kv_wide_kernel<CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(512), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
+    hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
     if (part != nullptr) {
         const long n = (long)a.B * a.T * a.Hkv * a.D, grid = (2 * n / 8 + 255) / 256;
         hipLaunchKernelGGL(fold_parts_kernel, dim3((unsigned)(grid > 8192 ? 8192 : grid)), dim3(256), 0, st, part, parts, n, (unsigned short*)dk, (unsigned short*)dv);
