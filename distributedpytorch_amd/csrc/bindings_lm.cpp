@@ -303,8 +303,9 @@ Tensor token_embedding(const Tensor& tok, const Tensor& w, const Tensor& w_lp, d
 
 // ---------------------------------------------------------------- distillation
 // -> loss [1], and the logits' gradient for an upstream gradient of 1 (undefined unless asked for)
-std::vector<Tensor> distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool want_grad) {
-    CHECK_ON(logits, logits); TORCH_CHECK(logits.is_contiguous() && logits.dim() == 2, "distill: logits [N, ld], contiguous");
+std::vector<Tensor> distill(const Tensor& logits_, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool want_grad) {
+    CHECK_ON(logits_, logits_); TORCH_CHECK(logits_.dim() == 2, "distill: logits [N, ld]");
+    const Tensor logits = flat16(logits_);                                     // rows lie on 16 bytes as those of the gradient do
     const bool bf = logits.scalar_type() == at::kBFloat16;
     TORCH_CHECK(bf || logits.scalar_type() == at::kFloat, "distill: logits must be bf16 or fp32");
     CHECK_ON(ids, logits); TORCH_CHECK(ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt), "distill: ids int64 or int32");
@@ -316,13 +317,12 @@ std::vector<Tensor> distill(const Tensor& logits, const Tensor& ids, const Tenso
     TORCH_CHECK(tau > 0.0, "distill: temperature");
     Guard guard(logits.device());
     const auto fopt = logits.options().dtype(at::kFloat);
-    Tensor loss = torch::empty({1}, fopt), rows = torch::empty({N}, fopt), d;
+    Tensor loss = torch::empty({1}, fopt), rows = torch::empty({dpa::distill_blocks(bf, N, ld)}, fopt), d;
     if (want_grad) d = torch::empty_like(logits);
     dpa::DistillArgs a{};
     a.logits = logits.data_ptr(); a.dlogits = want_grad ? d.data_ptr() : nullptr;
     a.ids = ids.data_ptr(); a.teacher = teacher.data_ptr<float>(); a.row_loss = rows.data_ptr<float>();
     a.N = N; a.ld = ld; a.V = (int)V; a.K = (int)K; a.ids64 = ids.scalar_type() == at::kLong;
-    a.aligned = (ld * (bf ? 2 : 4)) % 16 == 0 && on16(logits) && (!want_grad || on16(d));
     a.inv_tau = (float)(1.0 / tau);
     const double n = N > 0 ? (double)N : 1.0;
     a.grad_scale = (float)(tau / n);

@@ -5,216 +5,282 @@
 //   live entries gives 0;  loss = sum of the rows / N;   d loss / d z_j = tau / N (q_j - sum over k with id_k = j of p_k).
 //
 // Bound by memory: z is read once and its gradient written once, both by the forward call when a gradient will be asked
-// for.  A 1024-thread workgroup takes a row.  Rows of up to 65,536 bf16 (32,768 fp32) columns stay in registers between the
-// sweeps (maximum, sum, gradient); longer or unaligned ones are read again, from the caches where they fit.  The teacher's
-// p is formed by the first wave from LDS; its share of the gradient - at most K places of a row - is written over the
-// dense part behind a barrier, every place by all the entries that name it with the same sum, so that duplicates need
-// neither an order nor an atomic.  Row losses are folded in a fixed order by a second small kernel.
+// for.  A workgroup takes a row, held between the sweeps (maximum, sum of exponentials, gradient) as the 16-byte vectors
+// it was read in - rows of any length and start are covered by the aligned vectors over them, the two at the ends element
+// by element.  Four builds, chosen by how many vectors a row has (`launch`):
+//   up to 1024     256 threads, registers: short rows are all latency, and fewer waves meet at fewer, cheaper barriers;
+//   up to 8192     1024 threads, registers, as many workgroups as the CUs hold and the next row's loads in flight under this
+//                  row's arithmetic: one workgroup fills a CU here, and a row's load, sweeps and store would follow one
+//                  another (HELD_FIGURES);
+//   up to 25,600   1024 threads, 17 vectors a thread in registers and up to 8 in LDS (WIDE_FIGURES);
+//   beyond         read again for the gradient.
+// The teacher's p goes through LDS; its share of the gradient - at most K places of a row - is written over the dense part
+// behind a barrier, every place by all the entries that name it with the same sum, so that duplicates need neither an
+// order nor an atomic.  The loss is folded in a fixed order by a second small kernel.
 #include "common.h"
 #include "kernels.h"
 
 namespace dpa {
 namespace {
 
-constexpr int NT = 1024, KMAX = 1024;
+constexpr int KMAX = 1024;
 constexpr float NEG_BIG = -1.0e30f, LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]);
-template <> __device__ __forceinline__ void load8<unsigned short>(const unsigned short* p, float (&f)[8]) { const uint4 u = *(const uint4*)p; unpack8(u, f); }
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
-    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
 __device__ __forceinline__ float get1(const unsigned short* p) { return bf16_to_float(*p); }
 __device__ __forceinline__ float get1(const float* p) { return *p; }
 __device__ __forceinline__ void put1(unsigned short* p, float v) { *p = float_to_bf16(v); }
 __device__ __forceinline__ void put1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store8(unsigned short* p, const float (&f)[8]) { *(uint4*)p = pack8(f); }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
-    *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-}
+// 2^x as one instruction; arguments are <= 0 up to rounding, and what lies below the normal numbers may be 0
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = wave_reduce_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float m = red[0];
+template <typename T> struct Vec;
+template <> struct Vec<unsigned short> {
+    static constexpr int N = 8;
+    static constexpr unsigned NONE = 0xff80ff80u;                              // -inf, twice
+    __device__ static void unpack(const u32x4& r, float (&f)[8]) { unpack8(__builtin_bit_cast(uint4, r), f); }
+    __device__ static u32x4 pack(const float (&f)[8]) { return __builtin_bit_cast(u32x4, pack8(f)); }
+    __device__ static void set(u32x4& r, int j, unsigned short v) { r[j >> 1] = (j & 1) ? ((r[j >> 1] & 0xffffu) | ((unsigned)v << 16)) : ((r[j >> 1] & 0xffff0000u) | v); }
+};
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static constexpr unsigned NONE = 0xff800000u;
+    __device__ static void unpack(const u32x4& r, float (&f)[4]) {
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, red[w]);
-    return m;
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_reduce_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
+        for (int j = 0; j < 4; ++j) {
+            const unsigned u = r[j];                                           // a scalar first: a bit cast of the element itself reads element 0
+            f[j] = __builtin_bit_cast(float, u);
+        }
+    }
+    __device__ static u32x4 pack(const float (&f)[4]) {
+        return u32x4{__builtin_bit_cast(unsigned, f[0]), __builtin_bit_cast(unsigned, f[1]), __builtin_bit_cast(unsigned, f[2]), __builtin_bit_cast(unsigned, f[3])};
+    }
+    __device__ static void set(u32x4& r, int j, float v) { r[j] = __builtin_bit_cast(unsigned, v); }
+};
+
+// One row as the aligned 16-byte vectors over it: vector i holds elements N i - lead ..
+template <typename T>
+struct Row {
+    const T* z;
+    T* d;
+    int lead, V, ld;
+    __device__ __forceinline__ Row(const DistillArgs& a, long row) : z((const T*)a.logits + row * a.ld),
+        d(a.dlogits != nullptr ? (T*)a.dlogits + row * a.ld : nullptr), lead((int)(((uintptr_t)z & 15) / sizeof(T))), V(a.V), ld((int)a.ld) {}
+    // columns past the classes as -inf: they take part in nothing
+    __device__ __forceinline__ u32x4 load(int i) const {
+        const int e = i * Vec<T>::N - lead;
+        if (e >= 0 && e + Vec<T>::N <= V) return *(const u32x4*)(z + e);
+        u32x4 r = {Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE};
+        if (e < V && e > -Vec<T>::N)
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) s += red[w];
+            for (int j = 0; j < Vec<T>::N; ++j)
+                if (e + j >= 0 && e + j < V) Vec<T>::set(r, j, z[e + j]);
+        return r;
+    }
+    __device__ __forceinline__ void store(int i, const float (&f)[Vec<T>::N]) const {
+        const int e = i * Vec<T>::N - lead;
+        if (e >= 0 && e + Vec<T>::N <= ld) { *(u32x4*)(d + e) = Vec<T>::pack(f); return; }
+#pragma unroll
+        for (int j = 0; j < Vec<T>::N; ++j)
+            if (e + j >= 0 && e + j < ld) put1(d + e + j, f[j]);
+    }
+};
+
+// Two reductions over the workgroup in one exchange; every call in a row of `red` of its own, so one barrier each
+template <int NW, bool MAX>
+__device__ __forceinline__ float2 fold2(float x, float y, float2* red) {
+    x = MAX ? wave_reduce_max(x) : wave_reduce_sum(x);
+    y = MAX ? wave_reduce_max(y) : wave_reduce_sum(y);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(x, y);
+    __syncthreads();
+    float2 s = red[threadIdx.x % NW];
+#pragma unroll
+    for (int off = NW / 2; off > 0; off >>= 1) {
+        const float vx = __shfl_xor(s.x, off, 64), vy = __shfl_xor(s.y, off, 64);
+        s.x = MAX ? fmaxf(s.x, vx) : s.x + vx;
+        s.y = MAX ? fmaxf(s.y, vy) : s.y + vy;
+    }
     return s;
 }
 
-// live teacher entries of the row into LDS: ids_s (-1 where dead), p_s, logp_s.  Returns whether there are any.
-__device__ __forceinline__ bool teacher_row(const DistillArgs& a, long row, int* ids_s, float* p_s, float* lp_s, float* red) {
-    const int tid = threadIdx.x;
-    float t = 0.f;
-    bool live = false;
-    if (tid < a.K) {
-        const long id = a.ids64 ? (long)((const int64_t*)a.ids)[row * a.K + tid] : (long)((const int*)a.ids)[row * a.K + tid];
-        t = a.teacher[row * a.K + tid];
-        live = id >= 0 && id < a.V && !(t == -INFINITY);
-        ids_s[tid] = live ? (int)id : -1;
-    }
-    const float m = block_max(live ? t : -INFINITY, red);
-    const float x = live ? (t - m) * a.inv_tau : 0.f, e = live ? expf(x) : 0.f;
-    const float s = block_sum(e, red);
-    const bool any = __syncthreads_or(live);
-    if (tid < a.K) {
-        p_s[tid] = any ? e / s : 0.f;
-        lp_s[tid] = any && live ? x - logf(s) : 0.f;
-    }
-    __syncthreads();
-    return any;
-}
-
-// the row's loss (thread 0 writes it) and the teacher's places of the gradient; lse2 = log2 sum_j 2^(z_j c)
-template <typename T>
-__device__ __forceinline__ void finish_row(const DistillArgs& a, long row, const T* z, T* d, bool any, float c, float lse2, const int* ids_s, const float* p_s,
-                                           const float* lp_s, float* red) {
-    const int tid = threadIdx.x;
-    float term = 0.f;
-    if (any && tid < a.K && ids_s[tid] >= 0) {
-        const int id = ids_s[tid];
-        const float y = fmaf(get1(z + id), c, -lse2);                          // log2 q
-        term = p_s[tid] == 0.f ? 0.f : p_s[tid] * (lp_s[tid] - y * LN2);
-        if (d != nullptr) {
-            float same = 0.f;
-            for (int k = 0; k < a.K; ++k) same += ids_s[k] == id ? p_s[k] : 0.f;
-            put1(d + id, (exp2f(y) - same) * a.grad_scale);
+// KE = teacher entries per thread
+template <int KE> struct Teacher { int id[KE]; float t[KE], z[KE]; };
+template <int NT, int KE>
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, long row, Teacher<KE>& e) {
+#pragma unroll
+    for (int i = 0; i < KE; ++i) {
+        const int k = threadIdx.x + i * NT;
+        e.id[i] = -1;
+        e.t[i] = 0.f;
+        if (k < a.K) {
+            const long id = a.ids64 ? (long)((const int64_t*)a.ids)[row * a.K + k] : (long)((const int*)a.ids)[row * a.K + k];
+            e.t[i] = a.teacher[row * a.K + k];
+            e.id[i] = id >= 0 && id < a.V ? (int)id : -1;
         }
     }
-    const float sum = block_sum(term, red);
-    if (tid == 0) a.row_loss[row] = any ? sum : 0.f;
+}
+template <typename T, int KE>
+__device__ __forceinline__ void load_student(const T* z, Teacher<KE>& e) {
+#pragma unroll
+    for (int i = 0; i < KE; ++i) {
+        if (e.t[i] == -INFINITY) e.id[i] = -1;
+        e.z[i] = e.id[i] >= 0 ? get1(z + e.id[i]) : 0.f;
+    }
 }
 
-// NCH > 0: the row in registers, NCH chunks of 8 per thread; 0: any length and alignment, read again for each sweep
-template <typename T, int NCH>
+// NREG vectors a thread in registers; LDS: more of them in LDS; PIPE: the next row's loads go out before this row's sweeps;
+// NREG = 0: nothing is kept
+template <typename T, int NT, int NREG, bool LDS, bool PIPE>
 __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
-    __shared__ float red[NT / 64];
+    constexpr int N = Vec<T>::N, NW = NT / 64, KE = (KMAX + NT - 1) / NT, HELD = NREG > 0 ? NREG : 1;
+    extern __shared__ __attribute__((aligned(16))) u32x4 more[];               // LDS: vectors NREG .. of every thread
+    __shared__ float2 red[3][NW];
     __shared__ int ids_s[KMAX];
-    __shared__ float p_s[KMAX], lp_s[KMAX];
-    const int tid = threadIdx.x, V = a.V;
-    const long row = blockIdx.x, ld = a.ld;
-    const T* z = (const T*)a.logits + row * ld;
-    T* d = a.dlogits != nullptr ? (T*)a.dlogits + row * ld : nullptr;
+    __shared__ float p_s[KMAX];
+    const int tid = threadIdx.x;
     const float c = a.inv_tau * LOG2E;
-    if constexpr (NCH > 0) {
-        constexpr int W = sizeof(T) == 2 ? 1 : 2;                              // 16-byte words of a chunk
-        u32x4 raw[NCH][W];
+    u32x4 raw[HELD], nraw[PIPE ? HELD : 1];
+    Teacher<KE> te, nte;
+    float total = 0.f;
+    long row = blockIdx.x;
+    if (row < a.N) {
+        const Row<T> r(a, row);
+        load_teacher<NT>(a, row, te);
+        if (NREG > 0 && PIPE)
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int i = (tid + k * NT) * 8;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                raw[k][w] = u32x4{0, 0, 0, 0};
-                if (i < V) raw[k][w] = *(const u32x4*)((const unsigned char*)(z + i) + 16 * w);
-            }
-        }
-        const bool any = teacher_row(a, row, ids_s, p_s, lp_s, red);           // while the row is on its way
-        auto unpack = [&](int k, float (&f)[8]) {
-            const int i = (tid + k * NT) * 8;
-            if constexpr (sizeof(T) == 2) {
-                unpack8(__builtin_bit_cast(uint4, raw[k][0]), f);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const unsigned u = raw[k][j >> 2][j & 3];                  // a scalar first: a bit cast of the element itself reads element 0
-                    f[j] = __builtin_bit_cast(float, u);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = i + j < V ? f[j] : -INFINITY;
-        };
-        float m = NEG_BIG;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            float f[8];
-            unpack(k, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, f[j]);
-        }
-        m = block_max(m, red) * c;
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            float f[8];
-            unpack(k, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += exp2f(fmaf(f[j], c, -m));
-        }
-        const float lse2 = m + log2f(block_sum(s, red));
-        if (d != nullptr) {
-            const float g = any ? a.grad_scale : 0.f;
-#pragma unroll
-            for (int k = 0; k < NCH; ++k) {
-                const int i = (tid + k * NT) * 8;
-                if (i < ld) {
-                    float f[8];
-                    unpack(k, f);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = any && i + j < V ? exp2f(fmaf(f[j], c, -lse2)) * g : 0.f;
-                    store8(d + i, f);
-                }
-            }
-            __syncthreads();                                                   // the dense part is there before the teacher's places
-        }
-        finish_row<T>(a, row, z, d, any, c, lse2, ids_s, p_s, lp_s, red);
-    } else {
-        const bool any = teacher_row(a, row, ids_s, p_s, lp_s, red);
-        const int nv = a.aligned ? V / 8 : 0;
-        float m = NEG_BIG, s = 0.f;
-        for (int i = tid; i < nv; i += NT) {
-            float f[8];
-            load8(z + i * 8, f);
-            float lm = m;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lm = fmaxf(lm, f[j] * c);
-            s *= exp2f(m - lm);
-            m = lm;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += exp2f(fmaf(f[j], c, -m));
-        }
-        for (int i = nv * 8 + tid; i < V; i += NT) {
-            const float x = get1(z + i), lm = fmaxf(m, x * c);
-            s = s * exp2f(m - lm) + exp2f(fmaf(x, c, -lm));
-            m = lm;
-        }
-        const float mb = block_max(m, red);
-        const float lse2 = mb + log2f(block_sum(s * exp2f(m - mb), red));
-        if (d != nullptr) {
-            const float g = any ? a.grad_scale : 0.f;
-            for (int i = tid; i < nv; i += NT) {
-                float f[8];
-                load8(z + i * 8, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = any ? exp2f(fmaf(f[j], c, -lse2)) * g : 0.f;
-                store8(d + i * 8, f);
-            }
-            for (long i = nv * 8 + tid; i < ld; i += NT) put1(d + i, any && i < V ? exp2f(fmaf(get1(z + i), c, -lse2)) * g : 0.f);
-            __syncthreads();
-        }
-        finish_row<T>(a, row, z, d, any, c, lse2, ids_s, p_s, lp_s, red);
+            for (int k = 0; k < HELD; ++k) raw[k] = r.load(tid + k * NT);
+        load_student(r.z, te);
     }
+    for (; row < a.N; row += gridDim.x) {
+        const Row<T> r(a, row);
+        const int nv = (r.lead + r.ld + N - 1) / N;
+        const long next = row + gridDim.x;
+        if (NREG > 0 && !PIPE)
+#pragma unroll
+            for (int k = 0; k < HELD; ++k) raw[k] = r.load(tid + k * NT);
+        if (LDS)
+            for (int k = NREG; tid + k * NT < nv; ++k) more[(k - NREG) * NT + tid] = r.load(tid + k * NT);
+        if (next < a.N) {
+            load_teacher<NT>(a, next, nte);
+            if (NREG > 0 && PIPE) {
+                const Row<T> rn(a, next);
+#pragma unroll
+                for (int k = 0; k < HELD; ++k) nraw[k] = rn.load(tid + k * NT);
+            }
+        }
+        const auto sweep = [&](auto&& f) {                                     // f(vector number, its values)
+            if (NREG > 0) {
+#pragma unroll
+                for (int k = 0; k < HELD; ++k) {
+                    u32x4 q = raw[k];
+                    asm volatile("" : "+v"(q));                                // unpacked anew in every sweep, not kept as floats between them
+                    float v[N];
+                    Vec<T>::unpack(q, v);
+                    f(tid + k * NT, v);
+                }
+                if (LDS)
+                    for (int k = NREG; tid + k * NT < nv; ++k) {
+                        float v[N];
+                        Vec<T>::unpack(more[(k - NREG) * NT + tid], v);
+                        f(tid + k * NT, v);
+                    }
+            } else {
+                for (int i = tid; i < nv; i += NT) {
+                    float v[N];
+                    Vec<T>::unpack(r.load(i), v);
+                    f(i, v);
+                }
+            }
+        };
+        // maxima of the row and of the teacher's live entries (a NaN entry is live: the row's sums become NaN)
+        float m = NEG_BIG, s = 0.f, tm = -INFINITY;
+        bool live = false;
+#pragma unroll
+        for (int i = 0; i < KE; ++i)
+            if (te.id[i] >= 0) { live = true; tm = fmaxf(tm, te.t[i]); }
+        if (NREG > 0) {
+            sweep([&](int, float (&v)[N]) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
+            });
+        } else {                                                               // maximum and sum in one reading
+            sweep([&](int, float (&v)[N]) {
+                float lm = m;
+#pragma unroll
+                for (int j = 0; j < N; ++j) lm = fmaxf(lm, v[j]);
+                s *= fast_exp2((m - lm) * c);
+                m = lm;
+#pragma unroll
+                for (int j = 0; j < N; ++j) s += fast_exp2((v[j] - m) * c);
+            });
+        }
+        const float2 mm = fold2<NW, true>(m, tm, red[0]);
+        const float m2 = mm.x * c;
+        if (NREG > 0)
+            sweep([&](int, float (&v)[N]) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) s += fast_exp2(fmaf(v[j], c, -m2));
+            });
+        else
+            s *= fast_exp2((m - mm.x) * c);
+        float x[KE], ts = 0.f;
+#pragma unroll
+        for (int i = 0; i < KE; ++i) {
+            x[i] = te.id[i] >= 0 ? (te.t[i] - mm.y) * a.inv_tau : 0.f;
+            ts += te.id[i] >= 0 ? expf(x[i]) : 0.f;
+        }
+        const float2 ss = fold2<NW, false>(s, ts, red[1]);
+        const bool any = __syncthreads_or(live);                               // a row without a teacher gives nothing, whatever it holds
+        const float lse2 = m2 + log2f(ss.x);
+        float p[KE], term = 0.f;
+#pragma unroll
+        for (int i = 0; i < KE; ++i) {
+            const int k = tid + i * NT;
+            p[i] = te.id[i] >= 0 ? expf(x[i]) / ss.y : 0.f;
+            if (k < a.K) { ids_s[k] = te.id[i]; p_s[k] = p[i]; }
+            const float y = fmaf(te.z[i], c, -lse2);                           // log2 q
+            if (te.id[i] >= 0) term += p[i] == 0.f ? 0.f : p[i] * (x[i] - logf(ss.y) - y * LN2);
+        }
+        if (next < a.N) load_student((const T*)a.logits + next * a.ld, nte);
+        if (r.d != nullptr) {
+            const float g = a.grad_scale;
+            if (any)
+                sweep([&](int i, float (&v)[N]) {
+                    if (i >= nv) return;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[j] = fast_exp2(fmaf(v[j], c, -lse2)) * g;
+                    r.store(i, v);
+                });
+            else
+                for (int i = tid; i < nv; i += NT) {
+                    float v[N] = {};
+                    r.store(i, v);
+                }
+        }
+        term = fold2<NW, false>(term, 0.f, red[2]).x;                          // (and: the dense part and the teacher's p are there)
+        if (r.d != nullptr)
+#pragma unroll
+            for (int i = 0; i < KE; ++i)
+                if (te.id[i] >= 0) {
+                    float same = 0.f;
+                    for (int k = 0; k < a.K; ++k) same += ids_s[k] == te.id[i] ? p_s[k] : 0.f;
+                    put1(r.d + te.id[i], (fast_exp2(fmaf(te.z[i], c, -lse2)) - same) * a.grad_scale);
+                }
+        if (any) total += term;
+        __syncthreads();                                                       // ids_s and p_s are read
+        te = nte;
+        if (NREG > 0 && PIPE)
+#pragma unroll
+            for (int k = 0; k < HELD; ++k) raw[k] = nraw[k];
+    }
+    if (tid == 0) a.row_loss[blockIdx.x] = total;
 }
 
-// loss = scale * sum of the rows, one workgroup, fixed order
-__global__ __launch_bounds__(NT) void fold_rows_kernel(const float* __restrict__ row_loss, long n, float scale, float* __restrict__ loss) {
-    __shared__ float red[NT / 64];
+// loss = scale * sum of the workgroups' shares, fixed order
+__global__ __launch_bounds__(256) void fold_loss_kernel(const float* __restrict__ part, int n, float scale, float* __restrict__ loss) {
+    __shared__ float2 red[4];
     float s = 0.f;
-    for (long i = threadIdx.x; i < n; i += NT) s += row_loss[i];
-    s = block_sum(s, red);
+    for (int i = threadIdx.x; i < n; i += 256) s += part[i];
+    s = fold2<4, false>(s, 0.f, red).x;
     if (threadIdx.x == 0) *loss = s * scale;
 }
 
@@ -226,44 +292,67 @@ __global__ __launch_bounds__(256) void scale_grad_kernel(T* __restrict__ d, cons
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) put1(d + i, get1(d + i) * gs);
 }
 
-template <typename T>
-void launch(const DistillArgs& a, hipStream_t st) {
-    const int nch = (int)((a.ld + 8 * NT - 1) / (8 * NT));
-    const bool held = a.aligned && a.ld % 8 == 0 && nch <= (sizeof(T) == 2 ? 8 : 4);
-#define DPA_DISTILL(N_) hipLaunchKernelGGL((distill_kernel<T, N_>), dim3((unsigned)a.N), dim3(NT), 0, st, a)
-    if (!held) { DPA_DISTILL(0); return; }
-    if constexpr (sizeof(T) == 2) {
-        switch (nch) {
-            case 1: DPA_DISTILL(1); break;
-            case 2: DPA_DISTILL(2); break;
-            case 3: DPA_DISTILL(3); break;
-            case 4: DPA_DISTILL(4); break;
-            case 5: DPA_DISTILL(5); break;
-            case 6: DPA_DISTILL(6); break;
-            case 7: DPA_DISTILL(7); break;
-            default: DPA_DISTILL(8); break;
-        }
-    } else {
-        switch (nch) {
-            case 1: DPA_DISTILL(1); break;
-            case 2: DPA_DISTILL(2); break;
-            case 3: DPA_DISTILL(3); break;
-            default: DPA_DISTILL(4); break;
-        }
+template <typename T, int NT, int NREG, bool LDS, bool PIPE>
+void start(const DistillArgs& a, int blocks, int lds, hipStream_t st) {
+    if (LDS) {
+        static const hipError_t ok = hipFuncSetAttribute((const void*)distill_kernel<T, NT, NREG, LDS, PIPE>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 * 16);
+        (void)ok;
     }
-#undef DPA_DISTILL
+    hipLaunchKernelGGL((distill_kernel<T, NT, NREG, LDS, PIPE>), dim3((unsigned)blocks), dim3(NT), lds, st, a);
+}
+
+// 16-byte vectors that cover any row, its start anywhere in one
+template <typename T>
+long vectors(long ld) { return (ld + Vec<T>::N - 1) / Vec<T>::N + (ld % Vec<T>::N != 0); }
+
+template <typename T>
+int blocks_of(long N, long ld) {
+    const long v = vectors<T>(ld), cus = 256;
+    const long most = v <= 1024 ? 4096 : v <= 8192 ? (v <= 3072 ? 2 * cus : cus) : 4 * cus;
+    return (int)(N < most ? N : most);
+}
+
+template <typename T>
+void launch(const DistillArgs& a, int blocks, hipStream_t st) {
+    const long v = vectors<T>(a.ld);
+    if (v <= 1024) {
+        switch ((v + 255) / 256) {
+            case 1: start<T, 256, 1, false, false>(a, blocks, 0, st); break;
+            case 2: start<T, 256, 2, false, false>(a, blocks, 0, st); break;
+            case 3: start<T, 256, 3, false, false>(a, blocks, 0, st); break;
+            default: start<T, 256, 4, false, false>(a, blocks, 0, st); break;
+        }
+    } else if (v <= 8192) {
+        switch ((v + 1023) / 1024) {
+            case 1: case 2: start<T, 1024, 2, false, true>(a, blocks, 0, st); break;
+            case 3: start<T, 1024, 3, false, true>(a, blocks, 0, st); break;
+            case 4: start<T, 1024, 4, false, true>(a, blocks, 0, st); break;
+            case 5: start<T, 1024, 5, false, true>(a, blocks, 0, st); break;
+            case 6: start<T, 1024, 6, false, true>(a, blocks, 0, st); break;
+            case 7: start<T, 1024, 7, false, true>(a, blocks, 0, st); break;
+            default: start<T, 1024, 8, false, true>(a, blocks, 0, st); break;
+        }
+    } else if (v <= 25 * 1024) {
+        const long over = v - 17 * 1024;
+        start<T, 1024, 17, true, false>(a, blocks, over > 0 ? (int)((over + 1023) / 1024) * 1024 * 16 : 0, st);
+    } else {
+        start<T, 1024, 0, false, false>(a, blocks, 0, st);
+    }
 }
 
 }  // namespace
 
 int distill_max_entries() { return KMAX; }
 
+int distill_blocks(int is_bf16, long N, long ld) { return is_bf16 ? blocks_of<unsigned short>(N, ld) : blocks_of<float>(N, ld); }
+
 void distill(const DistillArgs& a, int is_bf16, float loss_scale, float* loss, hipStream_t st) {
-    if (a.N > 0) {
-        if (is_bf16) launch<unsigned short>(a, st);
-        else launch<float>(a, st);
+    const int blocks = distill_blocks(is_bf16, a.N, a.ld);
+    if (blocks > 0) {
+        if (is_bf16) launch<unsigned short>(a, blocks, st);
+        else launch<float>(a, blocks, st);
     }
-    hipLaunchKernelGGL(fold_rows_kernel, dim3(1), dim3(NT), 0, st, a.row_loss, a.N, loss_scale, loss);
+    hipLaunchKernelGGL(fold_loss_kernel, dim3(1), dim3(256), 0, st, a.row_loss, blocks, loss_scale, loss);
 }
 
 void scale_grad(void* d, int is_bf16, const float* g, long n, hipStream_t st) {

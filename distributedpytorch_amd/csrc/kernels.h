@@ -284,16 +284,17 @@ void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, 
                          int* sorted, float* partial, hipStream_t st);
 // distillation from a teacher's top logits (distill.hip)
 struct DistillArgs {
-    const void* logits;                    // [N, ld] bf16 or fp32
+    const void* logits;                    // [N, ld] bf16 or fp32, on 16 bytes
     void* dlogits;                         // same, or nullptr: no gradient
     const void* ids;                       // [N, K] int64 (ids64) or int32
     const float* teacher;                  // [N, K]
-    float* row_loss;                       // [N] scratch
+    float* row_loss;                       // [distill_blocks] scratch
     long N, ld;
-    int V, K, ids64, aligned;              // aligned: every row of both tensors on 16 bytes
+    int V, K, ids64;
     float inv_tau, grad_scale;             // 1 / tau, tau / N
 };
 int distill_max_entries();
+int distill_blocks(int is_bf16, long N, long ld);
 void distill(const DistillArgs& a, int is_bf16, float loss_scale /* tau^2 / N */, float* loss, hipStream_t st);
 void scale_grad(void* d, int is_bf16, const float* g, long n, hipStream_t st);   // d *= *g unless *g is 1
 // y = addend + x * keep(seed, offset, i) / (1 - p)  (bf16, n % 8 == 0; addend optional): element dropout with the mask
