@@ -65,8 +65,26 @@ struct Row {
     int lead, V, ld;
     __device__ __forceinline__ Row(const DistillArgs& a, long row) : z((const T*)a.logits + row * a.ld),
         d(a.dlogits != nullptr ? (T*)a.dlogits + row * a.ld : nullptr), lead((int)(((uintptr_t)z & 15) / sizeof(T))), V(a.V), ld((int)a.ld) {}
-    // columns past the classes as -inf: they take part in nothing
-    __device__ __forceinline__ u32x4 load(int i) const {
+    // columns past the classes as -inf: they take part in nothing.  WHOLE: rows are whole vectors, and where the caller is
+    // `sure` that vector i lies in the row the access stands in no branch - behind one the compiler no longer knows how many
+    // stores follow a load and waits for them all in front of the next row.
+    template <bool WHOLE>
+    __device__ __forceinline__ u32x4 load(int i, bool sure) const {
+        if (WHOLE) {
+            u32x4 r = {Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE};
+            const int e = i * Vec<T>::N;
+            if (sure || e < ld) r = *(const u32x4*)(z + e);
+            if (e + Vec<T>::N > V) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    constexpr int P = Vec<T>::N / 4;                           // values of a word
+                    const unsigned u = r[w], none = Vec<T>::NONE;
+                    if (P == 1) r[w] = e + w < V ? u : none;
+                    else r[w] = (e + 2 * w < V ? u & 0xffffu : none & 0xffffu) | (e + 2 * w + 1 < V ? u & 0xffff0000u : none & 0xffff0000u);
+                }
+            }
+            return r;
+        }
         const int e = i * Vec<T>::N - lead;
         if (e >= 0 && e + Vec<T>::N <= V) return *(const u32x4*)(z + e);
         u32x4 r = {Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE};
@@ -76,7 +94,12 @@ struct Row {
                 if (e + j >= 0 && e + j < V) Vec<T>::set(r, j, z[e + j]);
         return r;
     }
-    __device__ __forceinline__ void store(int i, const float (&f)[Vec<T>::N]) const {
+    template <bool WHOLE>
+    __device__ __forceinline__ void store(int i, const float (&f)[Vec<T>::N], bool sure) const {
+        if (WHOLE) {
+            if (sure || i * Vec<T>::N < ld) *(u32x4*)(d + i * Vec<T>::N) = Vec<T>::pack(f);
+            return;
+        }
         const int e = i * Vec<T>::N - lead;
         if (e >= 0 && e + Vec<T>::N <= ld) { *(u32x4*)(d + e) = Vec<T>::pack(f); return; }
 #pragma unroll
@@ -128,10 +151,10 @@ __device__ __forceinline__ void load_student(const T* z, Teacher<KE>& e) {
 }
 
 // NREG vectors a thread in registers; LDS: more of them in LDS; PIPE: the next row's loads go out before this row's sweeps;
-// NREG = 0: nothing is kept
-template <typename T, int NT, int NREG, bool LDS, bool PIPE>
+// NREG = 0: nothing is kept.  A row has more than NT (NREG - 1) vectors, with LDS more than 8 NT.
+template <typename T, int NT, int NREG, bool LDS, bool PIPE, bool WHOLE>
 __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
-    constexpr int N = Vec<T>::N, NW = NT / 64, KE = (KMAX + NT - 1) / NT, HELD = NREG > 0 ? NREG : 1;
+    constexpr int N = Vec<T>::N, NW = NT / 64, KE = (KMAX + NT - 1) / NT, HELD = NREG > 0 ? NREG : 1, SURE = LDS ? 8 : HELD - 1;
     extern __shared__ __attribute__((aligned(16))) u32x4 more[];               // LDS: vectors NREG .. of every thread
     __shared__ float2 red[3][NW];
     __shared__ int ids_s[KMAX];
@@ -147,7 +170,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         load_teacher<NT>(a, row, te);
         if (NREG > 0 && PIPE)
 #pragma unroll
-            for (int k = 0; k < HELD; ++k) raw[k] = r.load(tid + k * NT);
+            for (int k = 0; k < HELD; ++k) raw[k] = r.template load<WHOLE>(tid + k * NT, k < SURE);
         load_student(r.z, te);
     }
     for (; row < a.N; row += gridDim.x) {
@@ -156,18 +179,18 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         const long next = row + gridDim.x;
         if (NREG > 0 && !PIPE)
 #pragma unroll
-            for (int k = 0; k < HELD; ++k) raw[k] = r.load(tid + k * NT);
+            for (int k = 0; k < HELD; ++k) raw[k] = r.template load<WHOLE>(tid + k * NT, k < SURE);
         if (LDS)
-            for (int k = NREG; tid + k * NT < nv; ++k) more[(k - NREG) * NT + tid] = r.load(tid + k * NT);
+            for (int k = NREG; tid + k * NT < nv; ++k) more[(k - NREG) * NT + tid] = r.template load<WHOLE>(tid + k * NT, true);
         if (next < a.N) {
             load_teacher<NT>(a, next, nte);
             if (NREG > 0 && PIPE) {
                 const Row<T> rn(a, next);
 #pragma unroll
-                for (int k = 0; k < HELD; ++k) nraw[k] = rn.load(tid + k * NT);
+                for (int k = 0; k < HELD; ++k) nraw[k] = rn.template load<WHOLE>(tid + k * NT, k < SURE);
             }
         }
-        const auto sweep = [&](auto&& f) {                                     // f(vector number, its values)
+        const auto sweep = [&](auto&& f) {                                     // f(vector number, its values, whether the row surely has it)
             if (NREG > 0) {
 #pragma unroll
                 for (int k = 0; k < HELD; ++k) {
@@ -175,19 +198,19 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
                     asm volatile("" : "+v"(q));                                // unpacked anew in every sweep, not kept as floats between them
                     float v[N];
                     Vec<T>::unpack(q, v);
-                    f(tid + k * NT, v);
+                    f(tid + k * NT, v, k < SURE);
                 }
                 if (LDS)
                     for (int k = NREG; tid + k * NT < nv; ++k) {
                         float v[N];
                         Vec<T>::unpack(more[(k - NREG) * NT + tid], v);
-                        f(tid + k * NT, v);
+                        f(tid + k * NT, v, true);
                     }
             } else {
                 for (int i = tid; i < nv; i += NT) {
                     float v[N];
-                    Vec<T>::unpack(r.load(i), v);
-                    f(i, v);
+                    Vec<T>::unpack(r.template load<WHOLE>(i, true), v);
+                    f(i, v, true);
                 }
             }
         };
@@ -198,12 +221,12 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         for (int i = 0; i < KE; ++i)
             if (te.id[i] >= 0) { live = true; tm = fmaxf(tm, te.t[i]); }
         if (NREG > 0) {
-            sweep([&](int, float (&v)[N]) {
+            sweep([&](int, float (&v)[N], bool) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
             });
         } else {                                                               // maximum and sum in one reading
-            sweep([&](int, float (&v)[N]) {
+            sweep([&](int, float (&v)[N], bool) {
                 float lm = m;
 #pragma unroll
                 for (int j = 0; j < N; ++j) lm = fmaxf(lm, v[j]);
@@ -216,7 +239,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         const float2 mm = fold2<NW, true>(m, tm, red[0]);
         const float m2 = mm.x * c;
         if (NREG > 0)
-            sweep([&](int, float (&v)[N]) {
+            sweep([&](int, float (&v)[N], bool) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) s += fast_exp2(fmaf(v[j], c, -m2));
             });
@@ -244,16 +267,15 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         if (r.d != nullptr) {
             const float g = a.grad_scale;
             if (any)
-                sweep([&](int i, float (&v)[N]) {
-                    if (i >= nv) return;
+                sweep([&](int i, float (&v)[N], bool sure) {
 #pragma unroll
                     for (int j = 0; j < N; ++j) v[j] = fast_exp2(fmaf(v[j], c, -lse2)) * g;
-                    r.store(i, v);
+                    r.template store<WHOLE>(i, v, sure);
                 });
             else
                 for (int i = tid; i < nv; i += NT) {
                     float v[N] = {};
-                    r.store(i, v);
+                    r.template store<WHOLE>(i, v, true);
                 }
         }
         term = fold2<NW, false>(term, 0.f, red[2]).x;                          // (and: the dense part and the teacher's p are there)
@@ -292,13 +314,18 @@ __global__ __launch_bounds__(256) void scale_grad_kernel(T* __restrict__ d, cons
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) put1(d + i, get1(d + i) * gs);
 }
 
-template <typename T, int NT, int NREG, bool LDS, bool PIPE>
-void start(const DistillArgs& a, int blocks, int lds, hipStream_t st) {
+template <typename T, int NT, int NREG, bool LDS, bool PIPE, bool WHOLE>
+void start_one(const DistillArgs& a, int blocks, int lds, hipStream_t st) {
     if (LDS) {
-        static const hipError_t ok = hipFuncSetAttribute((const void*)distill_kernel<T, NT, NREG, LDS, PIPE>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 * 16);
+        static const hipError_t ok = hipFuncSetAttribute((const void*)distill_kernel<T, NT, NREG, LDS, PIPE, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 * 16);
         (void)ok;
     }
-    hipLaunchKernelGGL((distill_kernel<T, NT, NREG, LDS, PIPE>), dim3((unsigned)blocks), dim3(NT), lds, st, a);
+    hipLaunchKernelGGL((distill_kernel<T, NT, NREG, LDS, PIPE, WHOLE>), dim3((unsigned)blocks), dim3(NT), lds, st, a);
+}
+template <typename T, int NT, int NREG, bool LDS, bool PIPE>
+void start(const DistillArgs& a, int blocks, int lds, hipStream_t st) {
+    if (a.ld % Vec<T>::N == 0) start_one<T, NT, NREG, LDS, PIPE, true>(a, blocks, lds, st);
+    else start_one<T, NT, NREG, LDS, PIPE, false>(a, blocks, lds, st);
 }
 
 // 16-byte vectors that cover any row, its start anywhere in one
