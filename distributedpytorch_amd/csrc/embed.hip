@@ -20,16 +20,17 @@
 namespace dpa {
 namespace {
 
-constexpr int SORT_WAVES = 16, CHUNK = 64;
+constexpr int SORT_WAVES = 16, BATCH = 16, CHUNK = 64;
 
 template <typename I>
 __global__ __launch_bounds__(256) void token_embedding_fwd_kernel(const I* __restrict__ tok, const unsigned short* __restrict__ w, unsigned short* __restrict__ y,
                                                                   long n, int C, long V, float scale) {
-    const int nch = C / 8;
-    const long total = n * nch;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long row = i / nch;
-        const int ch = (int)(i - row * nch);
+    const int nch = C / 8, rows = nch >= 256 ? 1 : 256 / nch;
+    for (long r0 = (long)blockIdx.x * rows; r0 < n; r0 += (long)gridDim.x * rows)
+    for (int i = threadIdx.x; i < rows * nch; i += 256) {
+        const int dr = i / nch, ch = i - dr * nch;
+        const long row = r0 + dr;
+        if (row >= n) break;
         const long id = (long)tok[row];
         float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (id >= 0 && id < V) {
@@ -38,9 +39,13 @@ __global__ __launch_bounds__(256) void token_embedding_fwd_kernel(const I* __res
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= scale;
         }
-        *(uint4*)(y + i * 8) = pack8(f);
+        *(uint4*)(y + row * C + ch * 8) = pack8(f);
     }
 }
+
+// an id as 32 bits, -1 for one that no table of fewer than 2^31 rows has
+__device__ __forceinline__ int small_id(int id) { return id; }
+__device__ __forceinline__ int small_id(int64_t id) { return (unsigned long long)id < 0x7fffffffull ? (int)id : -1; }
 
 // order[]: positions sorted by (id, position); start[v] .. start[v + 1]: id v's part of it.  Workgroup b owns ids
 // [b * width, min(V, (b + 1) * width)); LDS: SORT_WAVES * width counters.
@@ -51,18 +56,30 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void sort_tokens_kernel(const I* _
     __shared__ int below_s[SORT_WAVES], scan_s[SORT_WAVES];
     __shared__ int carry;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long lo = (long)blockIdx.x * width;
-    const int own = (int)(V - lo < width ? V - lo : width);
+    const int lo = (int)blockIdx.x * width, own = (int)(V - lo < width ? V - lo : width);
     for (int i = tid; i < SORT_WAVES * width; i += 64 * SORT_WAVES) hist[i] = 0;
     __syncthreads();
     const int piece = ((n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
     const int p0 = wave * piece, p1 = p0 + piece < n ? p0 + piece : n;
     int below = 0;
     int* mine = hist + wave * width;
-    for (int p = p0; p < p1; p += 64) {
-        const long id = p + lane < p1 ? (long)tok[p + lane] : -1;
-        below += (id >= 0 && id < lo) ? 1 : 0;
-        if (id >= lo && id < lo + own) atomicAdd(&mine[(int)(id - lo)], 1);
+    // the list 64 x BATCH tokens at a time, all loads of a batch on their way before the first is looked at: one after
+    // the other they are a chain of L2 round trips (16,384 tokens: SORT_FIGURES)
+    int ids[BATCH];
+    const auto load = [&](int p) {
+        I t[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) t[i] = p + 64 * i + lane < p1 ? tok[p + 64 * i + lane] : (I)-1;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) ids[i] = small_id(t[i]);
+    };
+    for (int p = p0; p < p1; p += 64 * BATCH) {
+        load(p);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            below += (unsigned)ids[i] < (unsigned)lo ? 1 : 0;
+            if ((unsigned)(ids[i] - lo) < (unsigned)own) atomicAdd(&mine[ids[i] - lo], 1);
+        }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
@@ -106,25 +123,28 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void sort_tokens_kernel(const I* _
         if (tid == 64 * SORT_WAVES - 1) carry = before + inc;
     }
     __syncthreads();
-    for (int p = p0; p < p1; p += 64) {
-        const long id = p + lane < p1 ? (long)tok[p + lane] : -1;
-        const bool hit = id >= lo && id < lo + own;
-        unsigned long long left = __ballot(hit);
-        const int v = (int)(id - lo);
-        while (left != 0) {                               // one distinct id per turn
-            const int lead = __ffsll((long long)left) - 1;
-            const int u = __shfl(v, lead, 64);
-            const unsigned long long same = __ballot(hit && v == u) & left;
-            const int at = mine[u];
-            if (hit && v == u) {
-                const int to = at + __popcll(same & ((1ull << lane) - 1));
-                order[to] = p + lane;
-                sorted[to] = (int)id;
+    for (int p = p0; p < p1; p += 64 * BATCH) {
+        if (piece > 64 * BATCH) load(p);                  // (else it is still there)
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int v = ids[i] - lo, q = p + 64 * i + lane;
+            const bool hit = (unsigned)v < (unsigned)own;
+            unsigned long long left = __ballot(hit);
+            while (left != 0) {                           // one distinct id per turn
+                const int lead = __ffsll((long long)left) - 1;
+                const int u = __builtin_amdgcn_readlane(v, lead);
+                const unsigned long long same = __ballot(hit && v == u) & left;
+                const int at = mine[u];
+                if (hit && v == u) {
+                    const int to = at + __popcll(same & ((1ull << lane) - 1));
+                    order[to] = q;
+                    sorted[to] = ids[i];
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (lane == lead) mine[u] = at + __popcll(same);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                left &= ~same;
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (lane == lead) mine[u] = at + __popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            left &= ~same;
         }
     }
 }
@@ -175,11 +195,13 @@ __device__ __forceinline__ void add_rows(float (&acc)[8], const int* __restrict_
 template <bool ADD>
 __global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ order, const int* __restrict__ start, const unsigned short* __restrict__ dy,
                                                        const float* __restrict__ partial, float* __restrict__ dw, long V, int C, float scale) {
-    const int nch = C / 8;
-    const long total = V * nch;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long v = i / nch;
-        const int ch = (int)(i - v * nch);
+    // a workgroup takes `rows` rows at a time: only the place within them is divided, in 32 bits
+    const int nch = C / 8, rows = nch >= 256 ? 1 : 256 / nch;
+    for (long v0 = (long)blockIdx.x * rows; v0 < V; v0 += (long)gridDim.x * rows)
+    for (int i = threadIdx.x; i < rows * nch; i += 256) {
+        const int dv = i / nch, ch = i - dv * nch;
+        const long v = v0 + dv;
+        if (v >= V) break;
         const int s = start[v], e = start[v + 1];
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         const int c0 = (s + CHUNK - 1) / CHUNK, c1 = e / CHUNK;      // whole chunks of the segment
@@ -226,7 +248,8 @@ void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C
                        tok, (int)n, V, width, start, order, sorted);
     if (partial != nullptr)
         hipLaunchKernelGGL(sum_chunks_kernel, dim3((unsigned)(n / CHUNK)), dim3(256), 0, st, order, sorted, start, V, (const unsigned short*)dy, partial, C);
-    const unsigned blocks = blocks_for(V * (C / 8), 1 << 20);
+    const long rows = C / 8 >= 256 ? 1 : 256 / (C / 8);
+    const unsigned blocks = blocks_for((V + rows - 1) / rows * 256, 1 << 20);
     if (add)
         hipLaunchKernelGGL((sum_rows_kernel<true>), dim3(blocks), dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale);
     else
@@ -237,7 +260,8 @@ void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C
 
 void token_embedding_fwd(const void* tok, int tok64, const void* w, void* y, long n, int C, long V, float scale, hipStream_t st) {
     if (n == 0) return;
-    const unsigned blocks = blocks_for(n * (C / 8), 1 << 20);
+    const long rows = C / 8 >= 256 ? 1 : 256 / (C / 8);
+    const unsigned blocks = blocks_for((n + rows - 1) / rows * 256, 1 << 20);
     if (tok64)
         hipLaunchKernelGGL((token_embedding_fwd_kernel<int64_t>), dim3(blocks), dim3(256), 0, st, (const int64_t*)tok, (const unsigned short*)w, (unsigned short*)y, n, C, V, scale);
     else
