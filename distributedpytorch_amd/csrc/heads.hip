@@ -18,7 +18,7 @@
 namespace dpa {
 namespace {
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 4, AHEAD = 6;
 constexpr double INV_2PI = 0.15915494309189533577;
 
 // orders one lane's LDS accesses with another's of the same wave
@@ -93,27 +93,37 @@ __global__ __launch_bounds__(64 * WAVES) void heads_fwd_kernel(HeadsArgs a, unsi
     const int nh = a.Hq + a.Hkv;
     const long row = (long)(a.Hq + 2 * a.Hkv) * a.D;
     for (long tok = (long)blockIdx.x * WAVES + wave; tok < a.tokens; tok += (long)gridDim.x * WAVES) {
-        if (a.R > 0) make_angles(cs, a.inv_freq, a.R / 2, a.positions != nullptr ? a.positions[tok] : tok % a.T, lane);
-        wave_sync();
         const unsigned short* x = (const unsigned short*)a.qkv + tok * row;
-        for (int h0 = 0; h0 < nh; h0 += 64 / L) {
-            const int hd = h0 + sub;
-            const bool live = in && hd < nh;
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (live) { const uint4 u = *(const uint4*)(x + (long)hd * a.D + ch * 8); unpack8(u, v); }
-            const bool is_q = hd < a.Hq;
-            if (NORM) {
-                float s = 0.f;
+        for (int h0 = 0; h0 < nh; h0 += AHEAD * (64 / L)) {
+            uint4 u[AHEAD];                                // on their way while the angles are made
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s += v[i] * v[i];
-                const float r = rsqrtf(head_sum<L>(s) / (float)a.D + a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= r * (is_q ? wq[i] : wk[i]);
+            for (int i = 0; i < AHEAD; ++i) {
+                const int hd = h0 + i * (64 / L) + sub;
+                u[i] = make_uint4(0, 0, 0, 0);
+                if (in && hd < nh) u[i] = *(const uint4*)(x + (long)hd * a.D + ch * 8);
             }
-            if (a.R > 0) rotate8<INTER>(v, cs, ch, a.R, base, 1.f);
-            if (live) {
-                unsigned short* dst = is_q ? q + (tok * a.Hq + hd) * a.D : k + (tok * a.Hkv + hd - a.Hq) * a.D;
-                *(uint4*)(dst + ch * 8) = pack8(v);
+            if (h0 == 0 && a.R > 0) make_angles(cs, a.inv_freq, a.R / 2, a.positions != nullptr ? a.positions[tok] : tok % a.T, lane);
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int hd = h0 + i * (64 / L) + sub;
+                if (h0 + i * (64 / L) >= nh) break;
+                const bool live = in && hd < nh, is_q = hd < a.Hq;
+                float v[8];
+                unpack8(u[i], v);
+                if (NORM) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s += v[j] * v[j];
+                    const float r = rsqrtf(head_sum<L>(s) / (float)a.D + a.eps);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= r * (is_q ? wq[j] : wk[j]);
+                }
+                if (a.R > 0) rotate8<INTER>(v, cs, ch, a.R, base, 1.f);
+                if (live) {
+                    unsigned short* dst = is_q ? q + (tok * a.Hq + hd) * a.D : k + (tok * a.Hkv + hd - a.Hq) * a.D;
+                    *(uint4*)(dst + ch * 8) = pack8(v);
+                }
             }
         }
         wave_sync();
