@@ -63,7 +63,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("distillation_loss: teacher_logits get no gradient")
     K = teacher_ids.shape[-1]
-    logits, teacher_ids, teacher_logits = logits.reshape(-1, ld), teacher_ids.reshape(-1, K), teacher_logits.reshape(-1, K)
+    if logits.dim() != 2:                          # (a view is a node of its own in backward: none where none is needed)
+        logits, teacher_ids, teacher_logits = logits.reshape(-1, ld), teacher_ids.reshape(-1, K), teacher_logits.reshape(-1, K)
     if not _ext.use_hip(logits):
         return _plain(logits, teacher_ids, teacher_logits, n_classes, temperature)
     if logits.dtype not in (torch.bfloat16, torch.float32):
