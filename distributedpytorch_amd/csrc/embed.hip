@@ -179,52 +179,57 @@ __global__ __launch_bounds__(256) void sum_chunks_kernel(const int* __restrict__
     }
 }
 
-__device__ __forceinline__ void add_rows(float (&acc)[8], const int* __restrict__ order, int s, int e, const unsigned short* __restrict__ dy, int C, int ch) {
+__device__ __forceinline__ floatx4 four(const unsigned short* p) {
+    const uint2 u = *(const uint2*)p;
+    return floatx4{bf16_to_float(u.x & 0xffff), bf16_to_float(u.x >> 16), bf16_to_float(u.y & 0xffff), bf16_to_float(u.y >> 16)};
+}
+__device__ __forceinline__ void add_rows(floatx4 (&acc)[2], const int* __restrict__ order, int s, int e, const unsigned short* __restrict__ dy, int C, int c) {
 #pragma unroll 4
     for (int i = s; i < e; ++i) {
-        float f[8];
-        const uint4 u = *(const uint4*)(dy + (long)order[i] * C + ch * 8);
-        unpack8(u, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += f[j];
+        const unsigned short* p = dy + (long)order[i] * C + c;
+        acc[0] += four(p);
+        acc[1] += four(p + C / 2);
     }
 }
 
+// A thread has four channels in each half of the row: as many loads in flight as with eight together, and stores that leave no
+// gaps between lanes.  The rows are stored past the caches, which they would only fill (ROWS_FIGURES).
 // ADD: rows that some token names are added to dw (which another stream may be adding to as well: one atomic per element);
 // otherwise every row is written
 template <bool ADD>
 __global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ order, const int* __restrict__ start, const unsigned short* __restrict__ dy,
-                                                       const float* __restrict__ partial, float* __restrict__ dw, long V, int C, float scale) {
-    // a workgroup takes `rows` rows at a time: only the place within them is divided, in 32 bits
-    const int nch = C / 8, rows = nch >= 256 ? 1 : 256 / nch;
-    for (long v0 = (long)blockIdx.x * rows; v0 < V; v0 += (long)gridDim.x * rows)
+                                                       const float* __restrict__ partial, float* __restrict__ dw, long V, int C, float scale, int rows) {
+    // a workgroup takes `rows` rows: only the place within them is divided, in 32 bits
+    const int nch = C / 8;
+    const long v0 = (long)blockIdx.x * rows;
     for (int i = threadIdx.x; i < rows * nch; i += 256) {
-        const int dv = i / nch, ch = i - dv * nch;
+        const int dv = i / nch, c = (i - dv * nch) * 4;
         const long v = v0 + dv;
         if (v >= V) break;
         const int s = start[v], e = start[v + 1];
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         const int c0 = (s + CHUNK - 1) / CHUNK, c1 = e / CHUNK;      // whole chunks of the segment
         if (partial == nullptr || c0 >= c1) {
-            add_rows(acc, order, s, e, dy, C, ch);
+            add_rows(acc, order, s, e, dy, C, c);
         } else {
-            add_rows(acc, order, s, c0 * CHUNK, dy, C, ch);
+            add_rows(acc, order, s, c0 * CHUNK, dy, C, c);
 #pragma unroll 4
-            for (int c = c0; c < c1; ++c) {
-                const float4 x = *(const float4*)(partial + (long)c * C + ch * 8), y = *(const float4*)(partial + (long)c * C + ch * 8 + 4);
-                acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
-                acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+            for (int k = c0; k < c1; ++k) {
+                acc[0] += *(const floatx4*)(partial + (long)k * C + c);
+                acc[1] += *(const floatx4*)(partial + (long)k * C + c + C / 2);
             }
-            add_rows(acc, order, c1 * CHUNK, e, dy, C, ch);
+            add_rows(acc, order, c1 * CHUNK, e, dy, C, c);
         }
-        float* o = dw + v * C + ch * 8;
+        acc[0] *= scale;
+        acc[1] *= scale;
+        float* o = dw + v * C + c;
         if (ADD) {
             if (s < e)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) unsafeAtomicAdd(o + j, acc[j] * scale);
+                for (int j = 0; j < 8; ++j) unsafeAtomicAdd(o + (j & 3) + (j >> 2) * (C / 2), acc[j >> 2][j & 3]);
         } else {
-            *(float4*)o = make_float4(acc[0] * scale, acc[1] * scale, acc[2] * scale, acc[3] * scale);
-            *(float4*)(o + 4) = make_float4(acc[4] * scale, acc[5] * scale, acc[6] * scale, acc[7] * scale);
+            __builtin_nontemporal_store(acc[0], (floatx4*)o);
+            __builtin_nontemporal_store(acc[1], (floatx4*)(o + C / 2));
         }
     }
 }
@@ -248,12 +253,12 @@ void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C
                        tok, (int)n, V, width, start, order, sorted);
     if (partial != nullptr)
         hipLaunchKernelGGL(sum_chunks_kernel, dim3((unsigned)(n / CHUNK)), dim3(256), 0, st, order, sorted, start, V, (const unsigned short*)dy, partial, C);
-    const long rows = C / 8 >= 256 ? 1 : 256 / (C / 8);
-    const unsigned blocks = blocks_for((V + rows - 1) / rows * 256, 1 << 20);
+    const int rows = C / 8 >= 512 ? 1 : 512 / (C / 8);
+    const dim3 blocks((unsigned)((V + rows - 1) / rows));
     if (add)
-        hipLaunchKernelGGL((sum_rows_kernel<true>), dim3(blocks), dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale);
+        hipLaunchKernelGGL((sum_rows_kernel<true>), blocks, dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
     else
-        hipLaunchKernelGGL((sum_rows_kernel<false>), dim3(blocks), dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale);
+        hipLaunchKernelGGL((sum_rows_kernel<false>), blocks, dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
 }
 
 }  // namespace
