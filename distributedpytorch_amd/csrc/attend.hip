@@ -120,29 +120,33 @@ struct TileWalk {
 // instruction fills 1 KiB in lane order, so the image's swizzle goes into which 16 bytes of the row each lane asks for.
 // Rows past the last one are past the end of the descriptor and arrive as zeros; columns past D repeat the last eight (the
 // other operand of every product that sums over them is zero there).  Completion: tiles_landed(), then a barrier.
-template <int DH>
+template <int DH, int ROWS = TILE>
 struct TileDma {
     const unsigned char* base;           // row 0
-    unsigned step;                       // bytes of 64 rows' strides
+    unsigned step;                       // bytes of ROWS rows' strides
     unsigned whole, last;                // what a tile may read: a full one's bytes, the last one's
     unsigned off;                        // this lane's bytes in the tile's first rows
-    __device__ __forceinline__ TileDma(const unsigned short* g, long rs, int T, int D, int tid) : base((const unsigned char*)g) {
+    // zeros: columns past D are zeros as well (for a tile whose partner's are not)
+    __device__ __forceinline__ TileDma(const unsigned short* g, long rs, int T, int D, int tid, bool zeros = false) : base((const unsigned char*)g) {
         constexpr int CPR = DH / 8;
         const int row = tid / CPR, slot = tid % CPR;
         const int key = DH == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
         const unsigned rb = (unsigned)rs * 2;
         off = row * rb + 2 * min((slot ^ key) * 8, D - 8);
-        step = 64 * rb;
-        whole = 63 * rb + 2 * D;
-        last = ((T - 1) % TILE) * rb + 2 * D;
+        if (zeros && (slot ^ key) * 8 >= D) off = 0x80000000u;       // past any descriptor
+        step = ROWS * rb;
+        whole = (ROWS - 1) * rb + 2 * D;
+        last = ((T - 1) % ROWS) * rb + 2 * D;
     }
+    // rows ROWS j ..
     __device__ __forceinline__ void fetch(unsigned char* lds, int j, bool is_last, int wave) const {
+        constexpr int LOADS = ROWS * DH * 2 / 4096;                  // of 256 / (DH / 8) rows each: a multiple of 16, so `key` repeats
         const u32x4 words = buffer_words(base + (unsigned long long)step * (unsigned)j, is_last ? last : whole);
         unsigned o = off;
         asm volatile("" : "+v"(o));                                  // the sums below are formed here, not kept across the loop
 #pragma unroll
-        for (int i = 0; i < DH / 32; ++i)                            // 256 / (DH / 8) rows each: a multiple of 16, so `key` repeats
-            dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + i * (step / (DH / 32)));
+        for (int i = 0; i < LOADS; ++i)
+            dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + i * (step / LOADS));
     }
 };
 // 64 words (documents, statistics) into LDS by one wave, a word a lane; zeros from word `n` on
@@ -157,14 +161,14 @@ __device__ __forceinline__ void tiles_landed() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// rows of padding become zeros (docs: the tile's 64 document numbers in LDS)
-template <int DH>
+// rows of padding become zeros (docs: the tile's document numbers in LDS)
+template <int DH, int ROWS = TILE>
 __device__ __forceinline__ void clear_padding(unsigned char* lds, const int* docs, int tid) {
     constexpr int CPR = DH / 8, RSTEP = 256 / CPR;
     u32x4 zero = {0, 0, 0, 0};
     asm volatile("" : "+v"(zero));                                   // formed here, not kept across the loop
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) {
+    for (int i = 0; i < ROWS * DH * 2 / 4096; ++i) {
         const int row = tid / CPR + i * RSTEP;
         if (docs[row] < 0) *(u32x4*)(lds + row * DH * 2 + (tid % CPR) * 16) = zero;
     }
@@ -239,6 +243,24 @@ __device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, con
         }
 }
 
+// A run of N matrix products fed from LDS: read(i) is issued AHEAD products in front of use(i, fragments).  Left to itself the
+// compiler reads a fragment, waits for it and multiplies, one after the other.
+template <int N, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void feed(Read read, Use use) {
+    decltype(read(0)) f[AHEAD + 1];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = read(i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, f[i % (AHEAD + 1)]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+struct Frag3 { bf16x8 a, b, c; };
+struct Frag2 { bf16x8 a, b; };
+
 // Scores in base 2 from raw products.  `r` (cap only): 1 / (1 + e^{2x}), from which 1 - tanh^2 = 4 r (1 - r).
 struct ScoreMap { float c, k1, cap2; };       // scale log2 e;  2 scale log2 e / cap;  cap log2 e
 __device__ __forceinline__ ScoreMap score_map(const AttendArgs& a, bool cap) {
@@ -291,7 +313,7 @@ __device__ __forceinline__ unsigned doc_bits(const int* docs, int h, int mine) {
     unsigned m = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) m |= docs[4 * h + acc_row(r, 0)] == mine ? 1u << acc_row(r, 0) : 0u;
-    return m;
+    return mine >= 0 ? m : 0u;                                      // (padding sees no padding either)
 }
 __device__ __forceinline__ float pick(unsigned bits, int row, float x, float otherwise) {
     const int k = (int)(bits << (31 - row)) >> 31;
@@ -683,10 +705,10 @@ __device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, c
         }
 }
 
-template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
                                                                const float2* __restrict__ stats, KvOut o) {
-    constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
+    constexpr int DH = 64, KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
     __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];
     __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
@@ -790,6 +812,101 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_kv_kernel(Att
     store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
 }
 
+// The same at width 128.  Two accumulators of 32 keys x 128 channels and both stationary operands are 192 registers; with what
+// two waves per SIMD leave beside them every fragment is read, waited for and used before the next one is read
+// (WIDE_FIGURES).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
+// in a CU all the same, a stage is a half tile of 32 queries.
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout, const float2* __restrict__ stats, KvOut o) {
+    constexpr int DH = 128, ROWS = 32, KK = DH / 16, DI = DH / 32, TB = ROWS * DH * 2, SB = 2 * TB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB + BQ * DH * 2];   // two stages of queries and output gradients, then the values
+    __shared__ __attribute__((aligned(256))) float2 lds_ss[2][TILE];      // (64 words land at once; the half's own are in front)
+    __shared__ __attribute__((aligned(256))) int Qds[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kl = lane & 31, h = lane >> 5;
+    const FragAt<DH> frags(lane);
+    const int heads = o.heads, hq0 = blockIdx.x * heads, b = blockIdx.y, hk = hq0 / (a.Hq / a.Hkv);
+    const int T = a.T, k0 = blockIdx.z * BQ, kw0 = k0 + 32 * wave, key = kw0 + kl, keyc = min(key, T - 1);
+    const int halves = (T + ROWS - 1) / ROWS, tiles = (T + TILE - 1) / TILE;
+    {
+        const TileDma<DH, ROWS> vdma((const unsigned short*)a.v + b * a.vb + hk * a.vh, a.vt, T, a.D, tid, true);
+        for (int i = 0; i < BQ / ROWS; ++i)
+            if (k0 / ROWS + i < halves) vdma.fetch(smem + 2 * SB + i * TB, k0 / ROWS + i, k0 / ROWS + i == halves - 1, wave);
+    }
+    bf16x8 kf[KK];
+    load_frags<DH>((const unsigned short*)a.k + b * a.kb + hk * a.kh + (long)keyc * a.kt, h, a.D, kf);
+    const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
+    const int pre = seen_prefix(a, b);
+    const int kdoc = docs != nullptr ? docs[keyc] : 0;
+    const ScoreMap sm = score_map(a, CAP);
+    zero_unless<DH>(kdoc >= 0, kf);                                 // (a padded key's values reach its own column of dP only, which its mask zeroes)
+    floatx16 dKt[DI], dVt[DI];
+#pragma unroll
+    for (int di = 0; di < DI; ++di) { zero16(dKt[di]); zero16(dVt[di]); }
+    TileWalk<true> walk;
+    walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, k0, wave, k0 < pre ? 0 : k0 / TILE, tiles);
+    const int key_from = key < pre ? -(1 << 30) : key;
+
+    for (int head = hq0; head < hq0 + heads; ++head) {
+        const TileDma<DH, ROWS> qdma((const unsigned short*)a.q + b * a.qb + head * a.qh, a.qt, T, a.D, tid);
+        const TileDma<DH, ROWS> odma(dout + ((long)b * T * a.Hq + head) * a.D, (long)a.Hq * a.D, T, a.D, tid);
+        const float2* stats_b = stats + ((long)b * a.Hq + head) * T;
+        const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
+        if (head > hq0) walk.restart();
+        int n = 2 * walk.next();                                    // the half tile at hand; a tile's front half first
+#define DPA_FETCH_Q(S_)                                                                                                  \
+    if (n < halves) {                                                                                                    \
+        qdma.fetch(smem + (S_) * SB, n, n == halves - 1, wave);                                                          \
+        odma.fetch(smem + (S_) * SB + TB, n, n == halves - 1, wave);                                                     \
+        if (wave == 0) fetch_words(lds_ss[S_], stats_b + n * ROWS, 2L * (T - n * ROWS), lane);                           \
+        else if (wave == 1 && docs != nullptr) fetch_words(Qds[S_], docs + n * ROWS, T - n * ROWS, lane);                \
+    }
+        __syncthreads();                                            // the stages are free of the head before
+        DPA_FETCH_Q(0)
+        for (int stage = 0; n < halves; stage ^= 1) {
+            tiles_landed();
+            __syncthreads();
+            if (walk.pad) {
+                clear_padding<DH, ROWS>(smem + stage * SB, Qds[stage], tid);
+                clear_padding<DH, ROWS>(smem + stage * SB + TB, Qds[stage], tid);
+                __syncthreads();
+            }
+            const int qt0 = n * ROWS;
+            const bool go = walk.mine && (qt0 + ROWS - 1 >= kw0 || kw0 < pre), same = walk.whole;
+            n = (n & 1) == 0 && n + 1 < halves ? n + 1 : 2 * walk.next();
+            DPA_FETCH_Q(stage ^ 1)
+            if (!go) continue;                                      // wave-uniform
+            const bool full = same && (qt0 >= kw0 + 31 || kw0 + 31 < pre) && qt0 + ROWS <= T;
+            const FragAt<DH> fr = frags.at(stage * SB), fv = frags.at(2 * SB + wave * TB);
+            floatx16 S, dP;
+            zero16(S); zero16(dP);
+            feed<KK, 2>([&](int kk) { return Frag3{fr.rows(smem, 0, 0, kk), fr.rows(smem, TB, 0, kk), fv.rows(smem, 0, 0, kk)}; },
+                        [&](int kk, const Frag3& f) {
+                            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a, kf[kk], S, 0, 0, 0);
+                            dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b, f.c, dP, 0, 0, 0);
+                        });
+            key_side<CAP, BIAS>(S, dP, lds_ss[stage] + 4 * h, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - qt0 / TILE * TILE);
+            if (!full) {
+                unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
+                if (!same) bits &= doc_bits(Qds[stage], h, kdoc);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
+                    dP[r] = pick(bits, acc_row(r, 0), dP[r], 0.f);
+                }
+            }
+            const bf16x8 pb[2] = {pack_regs(S, 0), pack_regs(S, 1)}, dsb[2] = {pack_regs(dP, 0), pack_regs(dP, 1)};
+            feed<2 * DI, 2>([&](int i) { return Frag2{fr.cols(smem, TB, 0, i / DI, i % DI), fr.cols(smem, 0, 0, i / DI, i % DI)}; },
+                            [&](int i, const Frag2& f) {
+                                dVt[i % DI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a, pb[i / DI], dVt[i % DI], 0, 0, 0);
+                                dKt[i % DI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b, dsb[i / DI], dKt[i % DI], 0, 0, 0);
+                            });
+        }
+#undef DPA_FETCH_Q
+    }
+    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
+}
+
 // dk, dv [n] = the sum of their parts [parts][2][n] in order, rounded once (n a multiple of 8)
 __global__ __launch_bounds__(256) void fold_parts_kernel(const float* __restrict__ part, int parts, long n, unsigned short* __restrict__ dk,
                                                          unsigned short* __restrict__ dv) {
@@ -817,7 +934,8 @@ void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* 
                        (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
     const int parts = part != nullptr ? attend_kv_parts(a) : 1, heads = a.Hq / a.Hkv / parts;
     const KvOut o{(unsigned short*)dk, (unsigned short*)dv, part, heads};
-    hipLaunchKernelGGL((attend_bwd_kv_kernel<DH, CAP, BIAS>), dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
+    constexpr auto kv = DH == 64 ? attend_bwd_kv_kernel<CAP, BIAS> : attend_bwd_kv_wide_kernel<CAP, BIAS>;
+    hipLaunchKernelGGL(kv, dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
     if (part != nullptr) {
         const long n = (long)a.B * a.T * a.Hkv * a.D, grid = (2 * n / 8 + 255) / 256;
         hipLaunchKernelGGL(fold_parts_kernel, dim3((unsigned)(grid > 8192 ? 8192 : grid)), dim3(256), 0, st, part, parts, n, (unsigned short*)dk, (unsigned short*)dv);
