@@ -600,11 +600,11 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
             const FragAt<DH> fr = frags.at(stage * SB);
             floatx16 S, dP;
             zero16(S); zero16(dP);
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), qf[kk], S, 0, 0, 0);
-                dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, t2, kk), dof[kk], dP, 0, 0, 0);
-            }
+            feed<KK, 2>([&](int kk) { return Frag2{fr.rows(smem, 0, t2, kk), fr.rows(smem, TB, t2, kk)}; },
+                        [&](int kk, const Frag2& f) {
+                            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a, qf[kk], S, 0, 0, 0);
+                            dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b, dof[kk], dP, 0, 0, 0);
+                        });
             float c = sm.c, add = -lse_q;
             if (BIAS && !CAP && (kt0 + 31 <= qw0 || pre <= qw0)) {  // as in the forward
                 S = bf.add(S, 0);
@@ -632,14 +632,9 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
 #pragma unroll
                 for (int r = 0; r < 16; ++r) S[r] = pick(bits, acc_row(r, 0), S[r], 0.f);
             }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 dsb = pack_regs(S, s);
-#pragma unroll
-                for (int di = 0; di < DI; ++di)
-                    dQt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, t2, s, di), dsb,
-                                                                      dQt[di], 0, 0, 0);
-            }
+            const bf16x8 dsb[2] = {pack_regs(S, 0), pack_regs(S, 1)};
+            feed<2 * DI, 3>([&](int i) { return fr.cols(smem, 0, t2, i / DI, i % DI); },
+                            [&](int i, bf16x8 f) { dQt[i % DI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, dsb[i / DI], dQt[i % DI], 0, 0, 0); });
         }
     }
     if (q < T) store_cols(dq + orow, dQt, qdoc >= 0 ? (CAP ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
