@@ -149,11 +149,12 @@ struct TileDma {
             dma16<true>(__amdgpu_buffer_rsrc_t(), words, lds + i * 4096 + wave * 1024, o + i * (step / LOADS));
     }
 };
-// 64 words (documents, statistics) into LDS by one wave, a word a lane; zeros from word `n` on
-__device__ __forceinline__ void fetch_words(void* lds, const void* from, long n, int lane) {
+// 64 words (documents, statistics) into LDS by one wave, a word a lane; zeros from word `n` on (all of them for n <= 0: a row's
+// second 32 queries may not exist)
+__device__ __forceinline__ void fetch_words(void* lds, const void* from, int n, int lane) {
     typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
     const unsigned at = (unsigned)(unsigned long long)(lds_byte_ptr)(unsigned char*)lds;
-    const u32x4 words = buffer_words(from, (unsigned)(min(n, 64L) * 4));
+    const u32x4 words = buffer_words(from, (unsigned)__builtin_amdgcn_readfirstlane(min(max(n, 0), 64) * 4));
     asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(words), "s"(at) : "memory");
 }
 // every load that this wave has issued is done
@@ -745,7 +746,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
     if (j < walk.end) {                                                                                                  \
         qdma.fetch(smem + (S_) * SB, j, j == tiles - 1, wave);                                                                    \
         odma.fetch(smem + (S_) * SB + TB, j, j == tiles - 1, wave);                                                               \
-        if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2L * (T - j * TILE - 32 * wave), lane);  \
+        if (wave < 2) fetch_words(lds_ss[S_] + 32 * wave, stats_b + j * TILE + 32 * wave, 2 * (T - j * TILE - 32 * wave), lane);  \
         else if (wave == 2 && docs != nullptr) fetch_words(Qds[S_], docs + j * TILE, T - j * TILE, lane);                \
     }
         __syncthreads();                                            // the stages are free of the head before
@@ -853,7 +854,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a
     if (n < halves) {                                                                                                    \
         qdma.fetch(smem + (S_) * SB, n, n == halves - 1, wave);                                                          \
         odma.fetch(smem + (S_) * SB + TB, n, n == halves - 1, wave);                                                     \
-        if (wave == 0) fetch_words(lds_ss[S_], stats_b + n * ROWS, 2L * (T - n * ROWS), lane);                           \
+        if (wave == 0) fetch_words(lds_ss[S_], stats_b + n * ROWS, 2 * (T - n * ROWS), lane);                           \
         else if (wave == 1 && docs != nullptr) fetch_words(Qds[S_], docs + n * ROWS, T - n * ROWS, lane);                \
     }
         __syncthreads();                                            // the stages are free of the head before

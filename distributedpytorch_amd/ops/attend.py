@@ -60,6 +60,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     ``causal=False``; and, with ``documents [B,T]`` (int32, any numbering, sorted ones run fastest), only keys of the query's
     own document.  A token with a negative document number is padding: it sees nothing, is seen by nothing, its output and
     gradients are zero, and what its rows hold does not matter.
+    Rows that are not padding hold finite numbers: as in any product with probabilities of zero, a NaN or infinity there may
+    reach queries that do not see it.
 
     Gradients for ``q``, ``k``, ``v``; the rest are constants.  Sums, statistics and scores are fp32; probabilities and
     score gradients are rounded to bf16 for the matrix products that follow them, outputs and gradients once at the end.
