@@ -171,7 +171,8 @@ __global__ __launch_bounds__(64 * WAVES) void heads_bwd_kernel(HeadsArgs a, cons
                 float s = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s += n[i] * n[i];
-                const float r = rsqrtf(head_sum<L>(s) / (float)a.D + a.eps);
+                // lanes without a query or key head add nothing to the gains' sums (with eps = 0 their 1 / sqrt is infinite)
+                const float ms = head_sum<L>(s) / (float)a.D + a.eps, r = live && !is_v ? rsqrtf(ms) : 0.f;
                 float d = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {

@@ -293,6 +293,29 @@ def test_heads_only_one_output_used_and_strided_input():
         assert torch.equal(ga, gb) and ga.abs().sum() > 0
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 64), (3, 2, 40), (1, 1, 256)])
+def test_heads_without_eps(Hq, Hkv, D):
+    """eps = 0 divides by a head's own root mean square alone; lanes that hold no such head (values, places past the last one) must
+    not bring their 1 / 0 into the gains' gradients.  n is within 2^-20, as with eps; a sum of T H terms within its terms' sizes."""
+    T = 9
+    x, gs = _rand(1, T, (Hq + 2 * Hkv) * D, seed=5), [_rand(1, T, h, D, seed=6 + i) for i, h in enumerate((Hq, Hkv, Hkv))]
+    w = [1 + 0.3 * _rand(D, seed=9 + i, dtype=torch.float32) for i in range(2)]
+    xs, ws = x.to(DEV).requires_grad_(), [t.to(DEV).requires_grad_() for t in w]
+    got = torch.autograd.grad(ops.qk_norm_rotary(xs, Hq, Hkv, q_weight=ws[0], k_weight=ws[1], eps=0.0), (xs, *ws), [g.to(DEV) for g in gs])
+    X = x.double().view(1, T, -1, D)
+    n = X / X.square().mean(3, keepdim=True).sqrt()
+    for i, (a, b) in enumerate(((0, Hq), (Hq, Hq + Hkv))):
+        terms = gs[i].double() * n[:, :, a:b]
+        _within(got[1 + i], terms.sum((0, 1, 2)), 2.0 ** -18 * terms.abs().sum((0, 1, 2)), "dw")
+        gw = gs[i].double() * w[i].double()
+        r = n[:, :, a:b] / X[:, :, a:b]
+        d = (gw * n[:, :, a:b]).mean(3, keepdim=True)
+        ref = r * (gw - n[:, :, a:b] * d)
+        size = r.abs() * (gw.abs() + n[:, :, a:b].abs() * (gw * n[:, :, a:b]).abs().mean(3, keepdim=True))
+        _within(got[0].view(1, T, -1, D)[:, :, a:b], ref, U16 * ref.abs() + 2.0 ** -18 * size, "dqkv")
+    assert torch.equal(got[0].view(1, T, -1, D)[:, :, Hq + Hkv:].cpu(), gs[2])
+
+
 def test_heads_empty():
     w = torch.ones(16, device=DEV, requires_grad=True)
     x = torch.zeros(2, 0, 48, dtype=torch.bfloat16, device=DEV, requires_grad=True)
