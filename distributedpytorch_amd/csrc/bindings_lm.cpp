@@ -266,7 +266,7 @@ Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy_, int64_t V, doub
     CHECK_FLAT16(dy, dy, at::kBFloat16);
     CHECK_ON(tok, dy); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
     const int64_t C = dy.size(-1), n = tok.numel();
-    TORCH_CHECK(dy.numel() == n * C && C >= 8 && C % 8 == 0 && C < (1 << 24) && V >= 1 && V < (1ll << 31) - 1 && n < (1ll << 31) - 4096, "token_embedding_bwd: shapes");
+    TORCH_CHECK(dy.numel() == n * C && C >= 8 && C % 8 == 0 && C < (1 << 24) && V >= 1 && V < (1ll << 31) - 1 && n < (1ll << 30), "token_embedding_bwd: shapes");
     const bool t64 = tok64(tok), add = acc.has_value();
     Guard guard(dy.device());
     const auto fopt = dy.options().dtype(at::kFloat), iopt = dy.options().dtype(at::kInt);
