@@ -17,6 +17,8 @@
 // The teacher's p goes through LDS; its share of the gradient - at most K places of a row - is written over the dense part
 // behind a barrier, every place by all the entries that name it with the same sum, so that duplicates need neither an
 // order nor an atomic.  The loss is folded in a fixed order by a second small kernel.
+#include <stdexcept>
+#include <string>
 #include "common.h"
 #include "kernels.h"
 
@@ -316,9 +318,9 @@ __global__ __launch_bounds__(256) void scale_grad_kernel(T* __restrict__ d, cons
 
 template <typename T, int NT, int NREG, bool LDS, bool PIPE, bool WHOLE>
 void start_one(const DistillArgs& a, int blocks, int lds, hipStream_t st) {
-    if (LDS) {
-        static const hipError_t ok = hipFuncSetAttribute((const void*)distill_kernel<T, NT, NREG, LDS, PIPE, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 * 16);
-        (void)ok;
+    if (LDS) {                                                                 // for every call: the limit belongs to the current device
+        const hipError_t e = hipFuncSetAttribute((const void*)distill_kernel<T, NT, NREG, LDS, PIPE, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 * 16);
+        if (e != hipSuccess) throw std::runtime_error(std::string("distill: no LDS for a wide row: ") + hipGetErrorString(e));
     }
     hipLaunchKernelGGL((distill_kernel<T, NT, NREG, LDS, PIPE, WHOLE>), dim3((unsigned)blocks), dim3(NT), lds, st, a);
 }
@@ -335,7 +337,7 @@ long vectors(long ld) { return (ld + Vec<T>::N - 1) / Vec<T>::N + (ld % Vec<T>::
 template <typename T>
 int blocks_of(long N, long ld) {
     const long v = vectors<T>(ld), cus = 256;
-    const long most = v <= 1024 ? 4096 : v <= 8192 ? (v <= 3072 ? 2 * cus : cus) : 4 * cus;
+    const long most = v <= 1024 ? 4096 : v <= 8192 ? (v <= 3 * 1024 ? 2 * cus : cus) : 4 * cus;
     return (int)(N < most ? N : most);
 }
 
@@ -351,7 +353,7 @@ void launch(const DistillArgs& a, int blocks, hipStream_t st) {
         }
     } else if (v <= 8192) {
         switch ((v + 1023) / 1024) {
-            case 1: case 2: start<T, 1024, 2, false, true>(a, blocks, 0, st); break;
+            case 2: start<T, 1024, 2, false, true>(a, blocks, 0, st); break;
             case 3: start<T, 1024, 3, false, true>(a, blocks, 0, st); break;
             case 4: start<T, 1024, 4, false, true>(a, blocks, 0, st); break;
             case 5: start<T, 1024, 5, false, true>(a, blocks, 0, st); break;

@@ -38,7 +38,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     int32) names.  An entry is dead when its id lies outside ``[0, n_classes)`` or its logit is ``-inf`` (short lists are
     padded so); an id may come twice; a row without live entries (a prompt's) contributes zero loss and gradient.
 
-    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once), zero in the padding columns.  ``logits`` are not
+    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once, and once more by an upstream gradient other than 1), zero in the padding columns.  ``logits`` are not
     changed.  On the GPU: bf16 or fp32 logits, fp32 teacher logits, ``K`` up to 1024.
     """
     if logits.dim() < 1 or not logits.dtype.is_floating_point:
