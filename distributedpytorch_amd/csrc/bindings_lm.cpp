@@ -266,7 +266,7 @@ Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy_, int64_t V, doub
     CHECK_FLAT16(dy, dy, at::kBFloat16);
     CHECK_ON(tok, dy); TORCH_CHECK(tok.is_contiguous(), "token_embedding: tokens must be contiguous");
     const int64_t C = dy.size(-1), n = tok.numel();
-    TORCH_CHECK(dy.numel() == n * C && C >= 8 && C % 8 == 0 && C < (1 << 24) && V >= 1 && V < (1ll << 31) - 1 && n < (1ll << 30), "token_embedding_bwd: shapes");
+    TORCH_CHECK(dy.numel() == n * C && C >= 8 && C % 8 == 0 && C < (1 << 24) && V >= 1 && V < (1ll << 30) && n <= (1ll << 27), "token_embedding_bwd: shapes");
     const bool t64 = tok64(tok), add = acc.has_value();
     Guard guard(dy.device());
     const auto fopt = dy.options().dtype(at::kFloat), iopt = dy.options().dtype(at::kInt);
@@ -278,11 +278,11 @@ Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy_, int64_t V, doub
     } else {
         dw = torch::empty({V, C}, fopt);
     }
-    Tensor scratch = torch::empty({V + 1 + 2 * n}, iopt), partial;
+    Tensor scratch = torch::empty({2 * (V + 1) + 2 * n}, iopt), partial;
     const long chunks = dpa::token_embedding_chunks(n);
     if (chunks > 0) partial = torch::empty({chunks, C}, fopt);
-    int* start = scratch.data_ptr<int>();
-    dpa::token_embedding_bwd(tok.data_ptr(), t64, dy.data_ptr(), dw.data_ptr<float>(), add, n, (int)C, V, (float)scale, start, start + V + 1, start + V + 1 + n,
+    int* span = scratch.data_ptr<int>();
+    dpa::token_embedding_bwd(tok.data_ptr(), t64, dy.data_ptr(), dw.data_ptr<float>(), add, n, (int)C, V, (float)scale, span, span + 2 * (V + 1), span + 2 * (V + 1) + n,
                              chunks > 0 ? partial.data_ptr<float>() : nullptr, cur_stream());
     return dw;
 }

@@ -5,11 +5,13 @@
 //
 // Bound by memory: the forward reads a table row per token and writes one; the backward reads dy once and writes dW once.
 // Backward in two launches (three from 512 tokens on), no atomics, every sum in one fixed order:
-//   1. sort_tokens: a workgroup owns a range of ids.  It reads the whole token list twice - once to count its ids (and the
-//      tokens below its range, which is where its output begins, so that no workgroup waits for another), once to place
-//      them.  Each of its 16 waves owns a contiguous piece of the list and a histogram of its own; the histograms summed
-//      over waves and ids give every (wave, id) its place, and inside a wave equal ids are ranked by ballots, so the sort
-//      is stable.  Re-reading the list costs L2 traffic only; a sort by passes over digits would cost two launches a digit.
+//   1. sort_tokens: a workgroup owns every 256th run of 8 ids (vocabularies put their common words side by side, and a range of ids
+//      would be one workgroup's work; single ids would leave the rows' sums no neighbours to share cache lines with).  It reads the whole token list, counts its ids -
+//      and the tokens that groups before it own, which is where its output begins, so that no workgroup waits for another -
+//      and notes where they stand.  Each of its 16 waves owns a contiguous piece of the list and a histogram of its own; the
+//      histograms summed over waves and ids give every (wave, id) its place, and inside a wave equal ids are ranked by
+//      ballots, so the sort is stable.  Reading the list in every workgroup costs L2 traffic only; a sort by passes over
+//      digits would cost two launches a digit.
 //   2. sum_chunks: the sorted list in chunks of 64; a chunk that lies inside ONE id's segment is summed to a partial row.
 //      This is where frequent tokens (6 % of a text are its commonest one) are spread over the chip.
 //   3. sum_rows: a thread per 8 channels of every table row adds the row's entries - whole chunks through their partials - and
@@ -21,6 +23,8 @@ namespace dpa {
 namespace {
 
 constexpr int SORT_WAVES = 16, BATCH = 16, CHUNK = 64;
+constexpr int SIDE_BITS = 3;                  // ids that stay side by side: 2^3
+constexpr int OWN_BITS = 9, HELD = 448;       // ids of a workgroup at most 2^9; places that a wave notes: 28 KiB beside 32 of counters
 
 template <typename I>
 __global__ __launch_bounds__(256) void token_embedding_fwd_kernel(const I* __restrict__ tok, const unsigned short* __restrict__ w, unsigned short* __restrict__ y,
@@ -43,119 +47,123 @@ __global__ __launch_bounds__(256) void token_embedding_fwd_kernel(const I* __res
     }
 }
 
-// an id as 32 bits, -1 for one that no table of fewer than 2^31 rows has
-__device__ __forceinline__ int small_id(int id) { return id; }
-__device__ __forceinline__ int small_id(int64_t id) { return (unsigned long long)id < 0x7fffffffull ? (int)id : -1; }
-
-// order[]: positions sorted by (id, position); start[v] .. start[v + 1]: id v's part of it.  Workgroup b owns ids
-// [b * width, min(V, (b + 1) * width)); LDS: SORT_WAVES * width counters.
+// order[]: positions sorted by (group, id, position), sorted[]: what stands there; span[v]: id v's part of it, span[V].x: how
+// many tokens there are.  Workgroup b of 2^g owns the ids whose g bits above the last SIDE_BITS are b, at most `width`; LDS: SORT_WAVES * width counters.
 template <typename I>
-__global__ __launch_bounds__(64 * SORT_WAVES) void sort_tokens_kernel(const I* __restrict__ tok, int n, long V, int width,
-                                                                      int* __restrict__ start, int* __restrict__ order, int* __restrict__ sorted) {
-    extern __shared__ int hist[];                         // [SORT_WAVES][width], then this workgroup's scan
+__global__ __launch_bounds__(64 * SORT_WAVES) void sort_tokens_kernel(const I* __restrict__ tok, int n, unsigned V, int g, int width,
+                                                                      int2* __restrict__ span, int* __restrict__ order, int* __restrict__ sorted) {
+    extern __shared__ int hist[];                         // [SORT_WAVES][width]
+    __shared__ unsigned held[SORT_WAVES][HELD];           // (place in the wave's piece) << 9 | own id
     __shared__ int below_s[SORT_WAVES], scan_s[SORT_WAVES];
-    __shared__ int carry;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int lo = (int)blockIdx.x * width, own = (int)(V - lo < width ? V - lo : width);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // ids turned right by g + SIDE_BITS: the group on top, so that one comparison each finds the groups before and its own
+    const unsigned lo = blockIdx.x << (32 - g), last = lo + ((1u << (32 - g)) - 1);
     for (int i = tid; i < SORT_WAVES * width; i += 64 * SORT_WAVES) hist[i] = 0;
     __syncthreads();
     const int piece = ((n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
     const int p0 = wave * piece, p1 = p0 + piece < n ? p0 + piece : n;
-    int below = 0;
+    int below = 0, cnt = 0, resume = 0;                   // tokens noted; the first that no longer was
     int* mine = hist + wave * width;
-    // the list 64 x BATCH tokens at a time, all loads of a batch on their way before the first is looked at: one after
-    // the other they are a chain of L2 round trips (16,384 tokens: SORT_FIGURES)
-    int ids[BATCH];
-    const auto load = [&](int p) {
-        I t[BATCH];
+    // Tokens from `from` on: 64 x BATCH at a time, all loads of a batch on their way before the first is looked at - one after
+    // the other they are a chain of L2 round trips (16,384 tokens: 18 us against 11).
+    const auto scan = [&](int from, bool count) {
+        cnt = 0;
+        resume = p1;
+        for (int p = from; p < p1 && (count || resume == p1); p += 64 * BATCH) {
+            I t[BATCH];
+            if (p + 64 * BATCH <= p1) {                   // wave-uniform: no test per token
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) t[i] = p + 64 * i + lane < p1 ? tok[p + 64 * i + lane] : (I)-1;
+                for (int i = 0; i < BATCH; ++i) t[i] = tok[p + 64 * i + lane];
+            } else {
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) ids[i] = small_id(t[i]);
-    };
-    for (int p = p0; p < p1; p += 64 * BATCH) {
-        load(p);
+                for (int i = 0; i < BATCH; ++i) t[i] = p + 64 * i + lane < p1 ? tok[p + 64 * i + lane] : (I)-1;
+            }
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            below += (unsigned)ids[i] < (unsigned)lo ? 1 : 0;
-            if ((unsigned)(ids[i] - lo) < (unsigned)own) atomicAdd(&mine[ids[i] - lo], 1);
+            for (int i = 0; i < BATCH; ++i) {
+                const bool there = sizeof(I) == 8 ? (unsigned long long)t[i] < V : (unsigned)t[i] < V;
+                const unsigned x = __builtin_rotateright32((unsigned)t[i], (unsigned)(g + SIDE_BITS));
+                const bool hit = there && x >= lo && x <= last;
+                const unsigned long long hits = __ballot(hit);
+                if (count) below += __popcll(__ballot(there && x < lo));
+                if (hits == 0) continue;                  // wave-uniform
+                const unsigned v = ((unsigned)t[i] >> (g + SIDE_BITS) << SIDE_BITS) | ((unsigned)t[i] & ((1u << SIDE_BITS) - 1));
+                if (count && hit) atomicAdd(&mine[v], 1);
+                if (resume < p1) continue;
+                if (cnt + __popcll(hits) > HELD) { resume = p + 64 * i; continue; }
+                if (hit) held[wave][cnt + __popcll(hits & ((1ull << lane) - 1))] = ((unsigned)(p - p0 + 64 * i + lane) << OWN_BITS) | v;
+                cnt += __popcll(hits);
+            }
         }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
+    };
+    scan(p0, true);
     if (lane == 0) below_s[wave] = below;
     __syncthreads();
     int base = 0;
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) base += below_s[w];
-    // exclusive scan of the ids' totals, 1024 at a time; each (wave, id) counter becomes its first place
-    if (tid == 0) carry = base;
-    for (int i0 = 0; i0 < own; i0 += 64 * SORT_WAVES) {
-        const int i = i0 + tid;
-        int total = 0;
-        if (i < own)
+    // exclusive scan of the ids' totals (at most 2^9); each (wave, id) counter becomes its first place
+    const unsigned id = ((unsigned)tid >> SIDE_BITS << (g + SIDE_BITS)) | (blockIdx.x << SIDE_BITS) | (tid & ((1u << SIDE_BITS) - 1));
+    const bool owned = tid < width && id < V;
+    int total = 0;
+    if (owned)
 #pragma unroll
-            for (int w = 0; w < SORT_WAVES; ++w) total += hist[w * width + i];
-        int inc = total;
+        for (int w = 0; w < SORT_WAVES; ++w) total += hist[w * width + tid];
+    int inc = total;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int t = __shfl_up(inc, off, 64);
-            if (lane >= off) inc += t;
-        }
-        __syncthreads();                                  // scan_s and carry of the round before are read
-        if (lane == 63) scan_s[wave] = inc;
-        __syncthreads();
-        int before = carry;
-#pragma unroll
-        for (int w = 0; w < SORT_WAVES; ++w) before += w < wave ? scan_s[w] : 0;
-        int at = before + inc - total;
-        if (i < own) {
-            start[lo + i] = at;
-#pragma unroll
-            for (int w = 0; w < SORT_WAVES; ++w) {
-                const int c = hist[w * width + i];
-                hist[w * width + i] = at;
-                at += c;
-            }
-            if (lo + i == V - 1) start[V] = at;
-        }
-        __syncthreads();
-        if (tid == 64 * SORT_WAVES - 1) carry = before + inc;
+    for (int off = 1; off < 64; off <<= 1) {
+        const int t = __shfl_up(inc, off, 64);
+        if (lane >= off) inc += t;
     }
+    if (lane == 63) scan_s[wave] = inc;
     __syncthreads();
-    for (int p = p0; p < p1; p += 64 * BATCH) {
-        if (piece > 64 * BATCH) load(p);                  // (else it is still there)
+    int at = base + inc - total;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int v = ids[i] - lo, q = p + 64 * i + lane;
-            const bool hit = (unsigned)v < (unsigned)own;
+    for (int w = 0; w < SORT_WAVES; ++w) at += w < wave ? scan_s[w] : 0;
+    if (owned) {
+        span[id] = make_int2(at, at + total);
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            const int c = hist[w * width + tid];
+            hist[w * width + tid] = at;
+            at += c;
+        }
+    }
+    if (blockIdx.x == gridDim.x - 1 && tid == 64 * SORT_WAVES - 1) span[V].x = at;      // (nothing is left to add there)
+    __syncthreads();
+    for (;;) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i0 = 0; i0 < cnt; i0 += 64) {
+            const bool hit = i0 + lane < cnt;
+            const unsigned e = hit ? held[wave][i0 + lane] : 0u, v = e & ((1u << OWN_BITS) - 1);
+            int rank = 0, same_ids = 0;
             unsigned long long left = __ballot(hit);
             while (left != 0) {                           // one distinct id per turn
-                const int lead = __ffsll((long long)left) - 1;
-                const int u = __builtin_amdgcn_readlane(v, lead);
-                const unsigned long long same = __ballot(hit && v == u) & left;
-                const int at = mine[u];
-                if (hit && v == u) {
-                    const int to = at + __popcll(same & ((1ull << lane) - 1));
-                    order[to] = q;
-                    sorted[to] = ids[i];
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                if (lane == lead) mine[u] = at + __popcll(same);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                const unsigned u = __builtin_amdgcn_readlane(v, __ffsll((long long)left) - 1);
+                const unsigned long long same = __ballot(hit && v == u);
+                if (v == u) { rank = __popcll(same & ((1ull << lane) - 1)); same_ids = __popcll(same); }
                 left &= ~same;
             }
+            const int first = mine[v];
+            if (hit) {
+                order[first + rank] = p0 + (int)(e >> OWN_BITS);
+                sorted[first + rank] = (int)((v << g) | blockIdx.x);         // (told apart is all that they need)
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (hit && rank == same_ids - 1) mine[v] = first + same_ids;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+        if (resume >= p1) break;
+        scan(resume, false);
     }
 }
 
 // partial[c][C] = sum of the 64 rows of chunk c of the sorted list, where they all belong to one id
-__global__ __launch_bounds__(256) void sum_chunks_kernel(const int* __restrict__ order, const int* __restrict__ sorted, const int* __restrict__ start,
+__global__ __launch_bounds__(256) void sum_chunks_kernel(const int* __restrict__ order, const int* __restrict__ sorted, const int2* __restrict__ span,
                                                          long V, const unsigned short* __restrict__ dy, float* __restrict__ partial, int C) {
     __shared__ float red[4][64 * 8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int s = blockIdx.x * CHUNK;
-    if (s + CHUNK > start[V] || sorted[s] != sorted[s + CHUNK - 1]) return;
+    if (s + CHUNK > span[V].x || sorted[s] != sorted[s + CHUNK - 1]) return;
     const int nch = C / 8;
     for (int c0 = 0; c0 < nch; c0 += 64) {
         const int ch = c0 + lane;
@@ -197,7 +205,7 @@ __device__ __forceinline__ void add_rows(floatx4 (&acc)[2], const int* __restric
 // ADD: rows that some token names are added to dw (which another stream may be adding to as well: one atomic per element);
 // otherwise every row is written
 template <bool ADD>
-__global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ order, const int* __restrict__ start, const unsigned short* __restrict__ dy,
+__global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ order, const int2* __restrict__ span, const unsigned short* __restrict__ dy,
                                                        const float* __restrict__ partial, float* __restrict__ dw, long V, int C, float scale, int rows) {
     // a workgroup takes `rows` rows: only the place within them is divided, in 32 bits
     const int nch = C / 8;
@@ -206,7 +214,7 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ o
         const int dv = i / nch, c = (i - dv * nch) * 4;
         const long v = v0 + dv;
         if (v >= V) break;
-        const int s = start[v], e = start[v + 1];
+        const int s = span[v].x, e = span[v].y;
         floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         const int c0 = (s + CHUNK - 1) / CHUNK, c1 = e / CHUNK;      // whole chunks of the segment
         if (partial == nullptr || c0 >= c1) {
@@ -239,26 +247,29 @@ inline unsigned blocks_for(long threads, long cap) {
     return (unsigned)(b < 1 ? 1 : b > cap ? cap : b);
 }
 
-// ids per workgroup of the sort: 256 workgroups where that leaves each at most 512 (32 KiB of counters)
-inline int sort_width(long V) {
-    const long w = (V + 255) / 256;
-    return (int)(w > 512 ? 512 : w);
+// the most ids that a workgroup of 2^g has
+inline int sort_width(long V, int g) { return (int)((((V - 1) >> (g + SIDE_BITS)) + 1) << SIDE_BITS); }
+// workgroups of the sort as a power of two: 256, one to a CU, or as many as leave each 2^9 ids
+inline int sort_bits(long V) {
+    int g = 1;
+    while (((1l << SIDE_BITS) << g) < V && (g < 8 || sort_width(V, g) > (1 << OWN_BITS))) ++g;
+    return g;
 }
 
 template <typename I>
-void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C, long V, float scale, int* start, int* order, int* sorted,
+void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C, long V, float scale, int2* span, int* order, int* sorted,
                  float* partial, hipStream_t st) {
-    const int width = sort_width(V);
-    hipLaunchKernelGGL((sort_tokens_kernel<I>), dim3((unsigned)((V + width - 1) / width)), dim3(64 * SORT_WAVES), SORT_WAVES * width * sizeof(int), st,
-                       tok, (int)n, V, width, start, order, sorted);
+    const int g = sort_bits(V), width = sort_width(V, g);
+    hipLaunchKernelGGL((sort_tokens_kernel<I>), dim3(1u << g), dim3(64 * SORT_WAVES), SORT_WAVES * width * sizeof(int), st,
+                       tok, (int)n, (unsigned)V, g, width, span, order, sorted);
     if (partial != nullptr)
-        hipLaunchKernelGGL(sum_chunks_kernel, dim3((unsigned)(n / CHUNK)), dim3(256), 0, st, order, sorted, start, V, (const unsigned short*)dy, partial, C);
+        hipLaunchKernelGGL(sum_chunks_kernel, dim3((unsigned)(n / CHUNK)), dim3(256), 0, st, order, sorted, span, V, (const unsigned short*)dy, partial, C);
     const int rows = C / 8 >= 512 ? 1 : 512 / (C / 8);
     const dim3 blocks((unsigned)((V + rows - 1) / rows));
     if (add)
-        hipLaunchKernelGGL((sum_rows_kernel<true>), blocks, dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
+        hipLaunchKernelGGL((sum_rows_kernel<true>), blocks, dim3(256), 0, st, order, span, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
     else
-        hipLaunchKernelGGL((sum_rows_kernel<false>), blocks, dim3(256), 0, st, order, start, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
+        hipLaunchKernelGGL((sum_rows_kernel<false>), blocks, dim3(256), 0, st, order, span, (const unsigned short*)dy, partial, dw, V, C, scale, rows);
 }
 
 }  // namespace
@@ -275,10 +286,10 @@ void token_embedding_fwd(const void* tok, int tok64, const void* w, void* y, lon
 
 long token_embedding_chunks(long n) { return n >= 8 * CHUNK ? n / CHUNK : 0; }
 
-void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, int add, long n, int C, long V, float scale, int* start, int* order,
+void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, int add, long n, int C, long V, float scale, void* span, int* order,
                          int* sorted, float* partial, hipStream_t st) {
-    if (tok64) backward_of((const int64_t*)tok, dy, dw, add, n, C, V, scale, start, order, sorted, partial, st);
-    else backward_of((const int*)tok, dy, dw, add, n, C, V, scale, start, order, sorted, partial, st);
+    if (tok64) backward_of((const int64_t*)tok, dy, dw, add, n, C, V, scale, (int2*)span, order, sorted, partial, st);
+    else backward_of((const int*)tok, dy, dw, add, n, C, V, scale, (int2*)span, order, sorted, partial, st);
 }
 
 }  // namespace dpa

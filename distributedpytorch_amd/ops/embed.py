@@ -57,8 +57,8 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, weight_lp: torch
         raise TypeError(f"token_embedding: the fp32 master on the GPU, got {weight.dtype}")
     if C % 8 or C >= 1 << 24:
         raise ValueError(f"token_embedding: {C} channels: a multiple of 8 on the GPU")
-    if V >= 2 ** 31 - 1 or tokens.numel() >= 2 ** 30:                      # (a launch has fewer than 2^32 threads, and a chunk of 64 tokens 256)
-        raise ValueError("token_embedding: at most 2^31 - 2 rows and 2^30 - 1 tokens")
+    if V >= 2 ** 30 or tokens.numel() > 2 ** 27:
+        raise ValueError("token_embedding: at most 2^30 - 1 rows and 2^27 tokens")
     if weight_lp is None:
         from .conv import _lp
         weight_lp = _lp(weight, None)
