@@ -279,11 +279,11 @@ Tensor token_embedding_bwd(const Tensor& tok, const Tensor& dy_, int64_t V, doub
         dw = torch::empty({V, C}, fopt);
     }
     Tensor scratch = torch::empty({2 * (V + 1) + 2 * n}, iopt), partial;
-    const long chunks = dpa::token_embedding_chunks(n);
-    if (chunks > 0) partial = torch::empty({chunks, C}, fopt);
+    const long partials = dpa::token_embedding_partials(n);
+    if (partials > 0) partial = torch::empty({partials, C}, fopt);
     int* span = scratch.data_ptr<int>();
     dpa::token_embedding_bwd(tok.data_ptr(), t64, dy.data_ptr(), dw.data_ptr<float>(), add, n, (int)C, V, (float)scale, span, span + 2 * (V + 1), span + 2 * (V + 1) + n,
-                             chunks > 0 ? partial.data_ptr<float>() : nullptr, cur_stream());
+                             partials > 0 ? partial.data_ptr<float>() : nullptr, cur_stream());
     return dw;
 }
 

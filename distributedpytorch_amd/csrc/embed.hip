@@ -12,9 +12,9 @@
 //      histograms summed over waves and ids give every (wave, id) its place, and inside a wave equal ids are ranked by
 //      ballots, so the sort is stable.  Reading the list in every workgroup costs L2 traffic only; a sort by passes over
 //      digits would cost two launches a digit.
-//   2. sum_chunks: the sorted list in chunks of 64; a chunk that lies inside ONE id's segment is summed to a partial row.
-//      This is where frequent tokens (6 % of a text are its commonest one) are spread over the chip.
-//   3. sum_rows: a thread per 8 channels of every table row adds the row's entries - whole chunks through their partials - and
+//   2. sum_runs: the sorted list in chunks of 64; what a chunk holds of one id is summed to a partial row where that is 16
+//      tokens or more.  This is where frequent tokens (6 % of a text are its commonest one) are spread over the chip.
+//   3. sum_rows: a thread per 8 channels of every table row adds the row's entries - long runs through their partials - and
 //      writes the row, zeros where no token named it: the gradient needs no clearing beforehand.
 #include "common.h"
 #include "kernels.h"
@@ -22,7 +22,7 @@
 namespace dpa {
 namespace {
 
-constexpr int SORT_WAVES = 16, BATCH = 16, CHUNK = 64;
+constexpr int SORT_WAVES = 16, BATCH = 16, CHUNK = 64, LONG = 16;
 constexpr int SIDE_BITS = 3;                  // ids that stay side by side: 2^3
 constexpr int OWN_BITS = 9, HELD = 448;       // ids of a workgroup at most 2^9; places that a wave notes: 28 KiB beside 32 of counters
 
@@ -157,33 +157,45 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void sort_tokens_kernel(const I* _
     }
 }
 
-// partial[c][C] = sum of the 64 rows of chunk c of the sorted list, where they all belong to one id
-__global__ __launch_bounds__(256) void sum_chunks_kernel(const int* __restrict__ order, const int* __restrict__ sorted, const int2* __restrict__ span,
-                                                         long V, const unsigned short* __restrict__ dy, float* __restrict__ partial, int C) {
+// The sorted list in chunks of 64.  What a chunk holds of one id is a run; the runs of at least LONG tokens - at most
+// CHUNK / LONG to a chunk, told apart by which LONG of the chunk they begin in - are summed to partial rows of their own.
+__device__ __forceinline__ long partial_row(int first) { return first / LONG; }
+
+// partial[partial_row(first)][C] = sum of the run's rows
+__global__ __launch_bounds__(256) void sum_runs_kernel(const int* __restrict__ order, const int* __restrict__ sorted, const int2* __restrict__ span,
+                                                       long V, const unsigned short* __restrict__ dy, float* __restrict__ partial, int C) {
     __shared__ float red[4][64 * 8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int s = blockIdx.x * CHUNK;
-    if (s + CHUNK > span[V].x || sorted[s] != sorted[s + CHUNK - 1]) return;
+    const int s = blockIdx.x * CHUNK, n = min(span[V].x - s, CHUNK);
+    if (n < LONG) return;
+    const int id = sorted[s + min(lane, n - 1)], before = __shfl_up(id, 1, 64);
+    const unsigned long long heads = __ballot(lane == 0 || id != before) & (~0ull >> (64 - n));
     const int nch = C / 8;
-    for (int c0 = 0; c0 < nch; c0 += 64) {
-        const int ch = c0 + lane;
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (ch < nch) {
-#pragma unroll 8
-            for (int i = 0; i < CHUNK / 4; ++i) {
-                float f[8];
-                const uint4 u = *(const uint4*)(dy + (long)order[s + wave * (CHUNK / 4) + i] * C + ch * 8);
-                unpack8(u, f);
+    for (unsigned long long left = heads; left != 0; left &= left - 1) {
+        const int a = __ffsll((long long)left) - 1;
+        const unsigned long long rest = left & (left - 1);
+        const int b = rest != 0 ? __ffsll((long long)rest) - 1 : n;
+        if (b - a < LONG) continue;
+        for (int c0 = 0; c0 < nch; c0 += 64) {
+            const int ch = c0 + lane;
+            float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (ch < nch) {
+#pragma unroll 4
+                for (int i = a + wave; i < b; i += 4) {
+                    float f[8];
+                    const uint4 u = *(const uint4*)(dy + (long)order[s + i] * C + ch * 8);
+                    unpack8(u, f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[j] += f[j];
+                    for (int j = 0; j < 8; ++j) acc[j] += f[j];
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) red[wave][lane * 8 + j] = acc[j];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 512; i += 256)
-            if (c0 * 8 + i < C) partial[(long)blockIdx.x * C + c0 * 8 + i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
-        __syncthreads();
+            for (int j = 0; j < 8; ++j) red[wave][lane * 8 + j] = acc[j];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 512; i += 256)
+                if (c0 * 8 + i < C) partial[partial_row(s + a) * C + c0 * 8 + i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+            __syncthreads();
+        }
     }
 }
 
@@ -200,8 +212,17 @@ __device__ __forceinline__ void add_rows(floatx4 (&acc)[2], const int* __restric
     }
 }
 
+__device__ __forceinline__ void add_partial(floatx4 (&acc)[2], const float* __restrict__ partial, int first, int C, int c) {
+    const float* p = partial + partial_row(first) * C + c;
+    acc[0] += *(const floatx4*)p;
+    acc[1] += *(const floatx4*)(p + C / 2);
+}
+
 // A thread has four channels in each half of the row: as many loads in flight as with eight together, and stores that leave no
-// gaps between lanes.  The rows are stored past the caches, which they would only fill (ROWS_FIGURES).
+// gaps between lanes.  The rows are stored past the caches, which they would only fill (16,384 tokens over 50,304 x 768, inputs not
+// in cache: 65 us with both otherwise, 40 so, and 31 since no row waits for more than LONG - 1 single entries on either side;
+// storing the zeros of 50,304 x 768 alone takes 23).  Eight loads at once instead of four cost the waves that hide them (65,536
+// tokens: 104 against 89 us).
 // ADD: rows that some token names are added to dw (which another stream may be adding to as well: one atomic per element);
 // otherwise every row is written
 template <bool ADD>
@@ -216,17 +237,20 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(const int* __restrict__ o
         if (v >= V) break;
         const int s = span[v].x, e = span[v].y;
         floatx4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-        const int c0 = (s + CHUNK - 1) / CHUNK, c1 = e / CHUNK;      // whole chunks of the segment
-        if (partial == nullptr || c0 >= c1) {
-            add_rows(acc, order, s, e, dy, C, c);
-        } else {
-            add_rows(acc, order, s, c0 * CHUNK, dy, C, c);
+        // the run in the first chunk, whole chunks, the run in the last one
+        const int first = partial != nullptr ? min(e, (s / CHUNK + 1) * CHUNK) : s, last = max(first, e / CHUNK * CHUNK);
+        int from = s;
+        if (first - s >= LONG) {
+            add_partial(acc, partial, s, C, c);
+            from = first;
+        }
+        const int mid = partial != nullptr ? first : e;
+        add_rows(acc, order, from, mid, dy, C, c);
+        if (partial != nullptr) {
 #pragma unroll 4
-            for (int k = c0; k < c1; ++k) {
-                acc[0] += *(const floatx4*)(partial + (long)k * C + c);
-                acc[1] += *(const floatx4*)(partial + (long)k * C + c + C / 2);
-            }
-            add_rows(acc, order, c1 * CHUNK, e, dy, C, c);
+            for (int k = first; k < last; k += CHUNK) add_partial(acc, partial, k, C, c);
+            if (e - last >= LONG) add_partial(acc, partial, last, C, c);
+            else add_rows(acc, order, last, e, dy, C, c);
         }
         acc[0] *= scale;
         acc[1] *= scale;
@@ -263,7 +287,7 @@ void backward_of(const I* tok, const void* dy, float* dw, int add, long n, int C
     hipLaunchKernelGGL((sort_tokens_kernel<I>), dim3(1u << g), dim3(64 * SORT_WAVES), SORT_WAVES * width * sizeof(int), st,
                        tok, (int)n, (unsigned)V, g, width, span, order, sorted);
     if (partial != nullptr)
-        hipLaunchKernelGGL(sum_chunks_kernel, dim3((unsigned)(n / CHUNK)), dim3(256), 0, st, order, sorted, span, V, (const unsigned short*)dy, partial, C);
+        hipLaunchKernelGGL(sum_runs_kernel, dim3((unsigned)((n + CHUNK - 1) / CHUNK)), dim3(256), 0, st, order, sorted, span, V, (const unsigned short*)dy, partial, C);
     const int rows = C / 8 >= 512 ? 1 : 512 / (C / 8);
     const dim3 blocks((unsigned)((V + rows - 1) / rows));
     if (add)
@@ -284,7 +308,7 @@ void token_embedding_fwd(const void* tok, int tok64, const void* w, void* y, lon
         hipLaunchKernelGGL((token_embedding_fwd_kernel<int>), dim3(blocks), dim3(256), 0, st, (const int*)tok, (const unsigned short*)w, (unsigned short*)y, n, C, V, scale);
 }
 
-long token_embedding_chunks(long n) { return n >= 8 * CHUNK ? n / CHUNK : 0; }
+long token_embedding_partials(long n) { return n >= 8 * CHUNK ? (n + LONG - 1) / LONG : 0; }
 
 void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, int add, long n, int C, long V, float scale, void* span, int* order,
                          int* sorted, float* partial, hipStream_t st) {

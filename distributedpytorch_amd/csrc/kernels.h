@@ -278,8 +278,8 @@ int heads_partial_rows(long tokens);
 void heads_bwd(const HeadsArgs& a, const void* dq, const void* dk, const void* dv, void* dqkv, float* partial, float* dqw, float* dkw, hipStream_t st);
 // scaled token embedding and its gradient by sorted tokens (embed.hip); tok int64 (tok64) or int32, C % 8 == 0; backward: n <= 2^27, V < 2^30
 void token_embedding_fwd(const void* tok, int tok64, const void* w, void* y, long n, int C, long V, float scale, hipStream_t st);
-long token_embedding_chunks(long n);       // rows of `partial`; 0: it may be nullptr
-// span [V + 1] pairs, order [n], sorted [n], partial [chunks, C] are scratch; add: into dw, else dw is written whole
+long token_embedding_partials(long n);       // rows of `partial`; 0: it may be nullptr
+// span [V + 1] pairs, order [n], sorted [n], partial [partials, C] are scratch; add: into dw, else dw is written whole
 void token_embedding_bwd(const void* tok, int tok64, const void* dy, float* dw, int add, long n, int C, long V, float scale, void* span, int* order,
                          int* sorted, float* partial, hipStream_t st);
 // distillation from a teacher's top logits (distill.hip)

@@ -375,6 +375,35 @@ def test_token_embedding_forward_and_backward(case, dtype):
         assert torch.equal(dw, again)
 
 
+@pytest.mark.parametrize("kind,V,C,n", [("runs", 4000, 16, 0), ("runs", 300, 136, 0), ("one", 90, 8, 30000), ("low", 50304, 8, 40000),
+                                        ("low", 20, 24, 20000), ("late", 600, 8, 16384)])
+def test_token_embedding_gradient_of_frequent_tokens(kind, V, C, n):
+    """Ids that come in every number around 16 and 64, so that their entries end just in front of, on and behind the places where the
+    sums are cut, and lists in which a wave meets more of its workgroup's ids than it can note at once.  n terms in fp32, in any order:
+    within (n + 2) 2^-24 of the sum of their sizes."""
+    g = torch.Generator().manual_seed(V)
+    if kind == "runs":
+        tok = torch.cat([torch.full((c,), i * 7 % V) for i, c in enumerate((1, 15, 16, 17, 30, 32, 33, 48, 63, 64, 65, 79, 80, 81, 127, 128, 129, 16, 16, 200))])
+        tok = tok[torch.randperm(tok.numel(), generator=g)]
+    elif kind == "late":                                           # nothing, then a few ids of one workgroup without a pause
+        tok = torch.full((n,), -1)
+        tok[n // 2:] = torch.randint(0, 8, (n - n // 2,), generator=g)
+    elif kind == "one":
+        tok = torch.full((n,), 5)
+        tok[::1009] = 6
+    else:
+        tok = (torch.exp(torch.rand(n, generator=g, dtype=torch.float64) * math.log(V)) - 1).long()
+    dy = _rand(tok.numel(), C, seed=3)
+    w = torch.zeros(V, C, device=DEV, requires_grad=True)
+    dw, again = (torch.autograd.grad(ops.token_embedding(tok.to(DEV), w), w, dy.to(DEV))[0] for _ in range(2))
+    assert torch.equal(dw, again)
+    live = tok >= 0
+    at, rows = tok[live], dy.double()[live]
+    count = torch.bincount(at, minlength=V)[:, None].double()
+    zero = torch.zeros(V, C, dtype=torch.float64)
+    _within(dw, zero.index_add(0, at, rows), (count + 2) * U32 * zero.index_add(0, at, rows.abs()), "dw")
+
+
 def test_token_embedding_adds_into_an_installed_gradient_buffer():
     from distributedpytorch_amd.ops import sink
     V, C = 60, 32
