@@ -19,6 +19,12 @@
 //     rounded O alone costs dQ and dK as much accuracy as their own rounding does (3.8e-3 against 2.5e-3 of the norm at
 //     scores of standard deviation 8 under a cap of 30).
 //   * Rows behind a document number < 0 are staged as zeros: whatever a padded row holds reaches no product.
+//
+// Bound by the matrix cores and the vector instructions between their products (exponentials, masks, rounding), which a wave
+// does not overlap by itself.  One row of 8192, 16 query heads over 4 of width 128, with a bias: forward 360 us (760 TFLOP/s of
+// the visible half), dQ 405 (1020), dK / dV 530 + 23 for the parts (1000); a large matrix product reaches 1230 here.  Short
+// documents are bound by the tiles at their edges instead: 16 rows of 1024 in documents of 256, 12 heads of width 64: 52 / 51 /
+// 56 us, where their traffic alone would take 26 / 37 / 31.
 #include <math.h>
 #include <type_traits>
 #include "attn_tile.h"
@@ -325,6 +331,7 @@ __device__ __forceinline__ float pick(unsigned bits, int row, float x, float oth
 // Pipeline of the three kernels: two stages of LDS, each a 64-row tile of both streamed operands.  A stage's loads go out when
 // the stage in front of it is about to be used and have that tile's products to arrive in; one barrier per tile says both
 // that the tile is there and that nobody reads the stage that is filled next.
+// (Three stages at width 64 changed nothing: 54 / 52 / 58 us on the short documents above.)
 template <int DH> constexpr int stage_bytes() { return 2 * tile_bytes<DH>(); }
 // waves per SIMD: what the registers of the accumulators and the stationary operand leave (512 / 2 at width 128)
 template <int DH> constexpr int occupancy() { return DH == 64 ? 3 : 2; }
@@ -810,7 +817,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
 
 // The same at width 128.  Two accumulators of 32 keys x 128 channels and both stationary operands are 192 registers; with what
 // two waves per SIMD leave beside them every fragment is read, waited for and used before the next one is read
-// (WIDE_FIGURES).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
+// (one row of 8192, 16 heads over 4: 634 us, the form below 530).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
 // in a CU all the same, a stage is a half tile of 32 queries.
 template <bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout, const float2* __restrict__ stats, KvOut o) {
@@ -961,7 +968,9 @@ void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t 
 void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) { DPA_ATTEND_PICK(fwd_of, a, out, rest, lse2, st); }
 
 // Query heads of a group in how many workgroups: the fewest that give 1024 of them (4 per CU: their work differs by where
-// their keys stand), or one head each.  PARTS_FIGURES
+// their keys stand), or one head each.  At width 128, 16 heads over 4, whole
+// groups / 512 / 1024 workgroups took 1700 / 686 / 524 us on one row of 8192 and 565 / 249 / 220 on four of 2047; adding the parts
+// takes 14 us for two and 23 for four.
 int attend_kv_parts(const AttendArgs& a) {
     const int group = a.Hq / a.Hkv;
     const long wgs = (long)a.Hkv * a.B * ((a.T + BQ - 1) / BQ);

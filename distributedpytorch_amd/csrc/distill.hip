@@ -11,8 +11,9 @@
 //   up to 1024     256 threads, registers: short rows are all latency, and fewer waves meet at fewer, cheaper barriers;
 //   up to 8192     1024 threads, registers, as many workgroups as the CUs hold and the next row's loads in flight under this
 //                  row's arithmetic: one workgroup fills a CU here, and a row's load, sweeps and store would follow one
-//                  another (HELD_FIGURES);
-//   up to 25,600   1024 threads, 17 vectors a thread in registers and up to 8 in LDS (WIDE_FIGURES);
+//                  another (16,384 rows of 50,257 bf16: 1083 us so, 819 in flight; a large copy of the same bytes takes 690);
+//   up to 25,600   1024 threads, 17 vectors a thread in registers and up to 8 in LDS (2047 rows of 100,001 fp32: 425 us,
+//                  read again for the gradient 711);
 //   beyond         read again for the gradient.
 // The teacher's p goes through LDS; its share of the gradient - at most K places of a row - is written over the dense part
 // behind a barrier, every place by all the entries that name it with the same sum, so that duplicates need neither an
