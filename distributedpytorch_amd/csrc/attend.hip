@@ -254,6 +254,7 @@ __device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, con
 // compiler reads a fragment, waits for it and multiplies, one after the other.
 template <int N, int AHEAD, typename Read, typename Use>
 __device__ __forceinline__ void feed(Read read, Use use) {
+    __builtin_amdgcn_s_setprio(1);
     decltype(read(0)) f[AHEAD + 1];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
@@ -264,6 +265,7 @@ __device__ __forceinline__ void feed(Read read, Use use) {
         use(i, f[i % (AHEAD + 1)]);
     }
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
 }
 struct Frag3 { bf16x8 a, b, c; };
 struct Frag2 { bf16x8 a, b; };
@@ -398,6 +400,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         if (!go) continue;                                          // wave-uniform
         const FragAt<DH> fr = frags.at(stage * SB);
         floatx16 S[2];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             zero16(S[t2]);
@@ -405,6 +408,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
             for (int kk = 0; kk < KK; ++kk)
                 S[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), qf[kk], S[t2], 0, 0, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
         // y = c S + add, in base 2: the scale and what is the same for a lane's whole tile ride the exponent's multiply-add
         float c = sm.c, add = 0.f;
         if (BIAS && !CAP && (jt + TILE - 1 <= qw0 || pre <= qw0)) {  // wave-uniform: no visible key lies behind its query
@@ -485,6 +489,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
                 x[i] = __builtin_bit_cast(u32x4, d);
             }
         }
+        __builtin_amdgcn_s_setprio(1);
         for (int pass = full ? 1 : 0; pass < 2; ++pass) {
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2)
@@ -496,6 +501,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = pb[i];
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     if (q < T) {
         const bool empty = l == 0.f;                                // saw no key: output zero, and P = exp2(x - 1e30) = 0 in backward
