@@ -21,8 +21,8 @@
 //   * Rows behind a document number < 0 are staged as zeros: whatever a padded row holds reaches no product.
 //
 // Bound by the matrix cores and the vector instructions between their products (exponentials, masks, rounding), which a wave
-// does not overlap by itself.  One row of 8192, 16 query heads over 4 of width 128, with a bias: forward 360 us (760 TFLOP/s of
-// the visible half), dQ 405 (1020), dK / dV 530 + 23 for the parts (1000); a large matrix product reaches 1230 here.  Short
+// does not overlap by itself.  One row of 8192, 16 query heads over 4 of width 128, with a bias: forward 347 us (790 TFLOP/s of
+// the visible half), dQ 367 (1120), dK / dV 500 + 23 for the parts (1050); a large matrix product reaches 1230 here.  Short
 // documents are bound by the tiles at their edges instead: 16 rows of 1024 in documents of 256, 12 heads of width 64: 52 / 51 /
 // 56 us, where their traffic alone would take 26 / 37 / 31.
 #include <math.h>
@@ -252,6 +252,9 @@ __device__ __forceinline__ void store_cols(unsigned short* __restrict__ dst, con
 
 // A run of N matrix products fed from LDS: read(i) is issued AHEAD products in front of use(i, fragments).  Left to itself the
 // compiler reads a fragment, waits for it and multiplies, one after the other.
+// Here and in the other products a wave goes ahead of the SIMD's other waves: the matrix cores get the next product as soon as
+// they can take it, and the others' vector work fills what is left (one row of 8192, 16 heads over 4: forward 358 -> 347 us,
+// dQ 397 -> 367, dK / dV 525 -> 500; 16 heads of width 64: dK / dV 343 -> 330).
 template <int N, int AHEAD, typename Read, typename Use>
 __device__ __forceinline__ void feed(Read read, Use use) {
     __builtin_amdgcn_s_setprio(1);
@@ -789,11 +792,13 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
                 const FragAt<DH> fr = frags.at(stage * SB);
                 floatx16 S, dP;
                 zero16(S); zero16(dP);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
                     S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, 0, t2, kk), kf[kk], S, 0, 0, 0);
                     dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.rows(smem, TB, t2, kk), vf[kk], dP, 0, 0, 0);
                 }
+                __builtin_amdgcn_s_setprio(0);
                 const float2* ld4 = lds_s + 32 * t2 + 4 * h;
                 key_side<CAP, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
                 if (!full) {
@@ -805,6 +810,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
                         dP[r] = pick(bits, acc_row(r, 0), dP[r], 0.f);
                     }
                 }
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const bf16x8 pb = pack_regs(S, s), dsb = pack_regs(dP, s);
@@ -814,6 +820,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
                         dKt[di] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.cols(smem, 0, t2, s, di), dsb, dKt[di], 0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
             }
         }
 #undef DPA_FETCH_Q
@@ -823,7 +830,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
 
 // The same at width 128.  Two accumulators of 32 keys x 128 channels and both stationary operands are 192 registers; with what
 // two waves per SIMD leave beside them every fragment is read, waited for and used before the next one is read
-// (one row of 8192, 16 heads over 4: 634 us, the form below 530).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
+// (one row of 8192, 16 heads over 4: 634 us, the form below 500).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
 // in a CU all the same, a stage is a half tile of 32 queries.
 template <bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout, const float2* __restrict__ stats, KvOut o) {
@@ -975,7 +982,8 @@ void attend_fwd(const AttendArgs& a, void* out, void* rest, float* lse2, hipStre
 
 // Query heads of a group in how many workgroups: the fewest that give 1024 of them (4 per CU: their work differs by where
 // their keys stand), or one head each.  At width 128, 16 heads over 4, whole
-// groups / 512 / 1024 workgroups took 1700 / 686 / 524 us on one row of 8192 and 565 / 249 / 220 on four of 2047; adding the parts
+// groups / 512 / 1024 workgroups took 1700 / 686 / 524 us on one row of 8192 and 565 / 249 / 220 on four of 2047
+// (as it was when this was chosen); adding the parts
 // takes 14 us for two and 23 for four.
 int attend_kv_parts(const AttendArgs& a) {
     const int group = a.Hq / a.Hkv;
