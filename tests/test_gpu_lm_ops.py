@@ -585,6 +585,80 @@ def test_pass_on_another_stream_and_in_replayed_graphs(which):
                 t.fill_(7)                          # a replay has to write everything again
 
 
+def _large_passes():
+    """As `_passes`, through the builds that long and wide inputs take."""
+    q, k, v, do = (_rand(1, 1100, h, 128, seed=s).to(DEV) for s, h in enumerate((8, 2, 2, 8)))
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    slopes = torch.linspace(0.01, 0.2, 8, device=DEV)
+
+    def parts():                                    # key heads' gradients by parts
+        out = ops.attention(q, k, v, slopes=slopes)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), do))
+    tok = torch.zeros(24000, dtype=torch.int32)     # more of one workgroup's tokens than a wave notes at once
+    tok[::7] = torch.arange(len(tok[::7]), dtype=torch.int32) % 8
+    tok = tok.to(DEV)
+    tab = _rand(50, 64, seed=8, dtype=torch.float32).to(DEV).requires_grad_()
+    dy = _rand(24000, 64, seed=9).to(DEV)
+
+    def often():
+        y = ops.token_embedding(tok, tab, scale=0.5)
+        return (y.detach(), *torch.autograd.grad(y, tab, dy))
+    passes = {"parts": parts, "often": often}
+    for name, V in (("held", 20001), ("lds", 70001), ("again", 110000)):
+        z = _rand(5, V, seed=V, dtype=torch.float32).to(DEV).requires_grad_()
+        ids, t = (a.to(DEV) for a in _teacher(5, V, 20, 11))
+
+        def distil(z=z, ids=ids, t=t):
+            loss = ops.distillation_loss(z, ids, t, temperature=2.0)
+            return (loss.detach(), *torch.autograd.grad(loss, z))
+        passes[name] = distil
+    return passes
+
+
+@pytest.mark.parametrize("which", ["parts", "often", "held", "lds", "again"])
+def test_large_pass_on_two_streams_at_once_and_in_a_replayed_graph(which):
+    go = _large_passes()[which]
+    want = [t.clone() for t in go()]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):                              # nothing waits between the two: each call has its own workspace
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(go())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        outs = go()
+    for _ in range(3):
+        graph.replay()
+        eager = go()
+        torch.cuda.synchronize()
+        got += [[t.clone() for t in outs], eager]
+        for t in outs:
+            t.fill_(7)
+    for one in got:
+        for a, b in zip(one, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["attend", "heads", "embed", "distil"])
+def test_second_backward_through_a_kept_graph(which):
+    """The same gradient again, also after the first one was changed in place."""
+    x = {"attend": lambda: _rand(1, 50, 2, 64), "heads": lambda: _rand(1, 5, 192), "embed": lambda: _rand(9, 8, dtype=torch.float32),
+         "distil": lambda: _rand(3, 20)}[which]().to(DEV).requires_grad_()
+    y = {"attend": lambda: ops.attention(x, x, x), "heads": lambda: ops.qk_norm_rotary(x, 1, inv_freq=ops.rotary_frequencies(64, device=DEV))[0],
+         "embed": lambda: ops.token_embedding(torch.tensor([1, 2, 1], device=DEV), x),
+         "distil": lambda: ops.distillation_loss(x, torch.tensor([[1], [2], [3]], device=DEV), torch.zeros(3, 1, device=DEV))}[which]()
+    g = torch.full_like(y, 0.5)
+    (first,) = torch.autograd.grad(y, x, g, retain_graph=True)
+    kept = first.clone()
+    first.fill_(3)
+    for _ in range(2):
+        (again,) = torch.autograd.grad(y, x, g, retain_graph=True)
+        assert torch.equal(again, kept)
+
+
 @pytest.mark.parametrize("which", ["attend", "heads", "embed", "distil"])
 def test_no_second_derivative(which):
     x = {"attend": lambda: _rand(1, 5, 2, 64), "heads": lambda: _rand(1, 5, 192), "embed": lambda: _rand(9, 8, dtype=torch.float32),
