@@ -449,10 +449,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[t2][r]);
         mx = xhalf_max(mx);
-        const float peak = BIAS && !CAP ? fmaf(mx, c, add) : CAP ? mx : mx * c;
-        // In tiles that are seen whole the reference follows the peak only when that has run 2^8 away from it: any reference serves
-        // as long as sums and P stay in range, and each step multiplies the whole accumulator.
-        const float mn = full && peak <= m + 8.f ? m : fmaxf(m, peak);
+        const float peak = BIAS && !CAP ? fmaf(mx, c, add) : CAP ? mx : mx * c, mn = fmaxf(m, peak);
         const bool grew = mn > m;
         float off = BIAS && !CAP ? add - mn : -mn;
         if (!full) {
