@@ -161,7 +161,7 @@ __device__ __forceinline__ void fetch_words(void* lds, const void* from, int n, 
     typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
     const unsigned at = (unsigned)(unsigned long long)(lds_byte_ptr)(unsigned char*)lds;
     const u32x4 words = buffer_words(from, (unsigned)__builtin_amdgcn_readfirstlane(min(max(n, 0), 64) * 4));
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(words), "s"(at) : "memory");
+    dma_lds4(words, at, lane * 4);
 }
 // every load that this wave has issued is done
 __device__ __forceinline__ void tiles_landed() {

@@ -73,7 +73,21 @@ __device__ __forceinline__ float gelu_tanh_grad(float x) {
     return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * du;
 }
 
-// 16 B per lane from a buffer descriptor straight into LDS (lane-linear destination from the wave-uniform `lds`).
+// 16 or 4 B per lane from a buffer descriptor straight into LDS (lane-linear destination from the wave-uniform LDS address), issued
+// from inline assembly: the only places that write M0 by hand.  The load reads M0, and a scalar write of M0 has to be one wait
+// state old by then; the compiler puts that s_nop in front of its own builtin and cannot look into an asm block.  The descriptor's
+// words are SALU results wherever dma_lds16 is used (its count is formed from kernel arguments); dma_lds4 is given counts that went
+// through v_readfirstlane, and a vector instruction's SGPR has to be five wait states old when a load reads it.
+__device__ __forceinline__ void dma_lds16(u32x4 rs4, unsigned lds_addr, unsigned voffset) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(voffset), "s"(rs4), "s"(lds_addr) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_lds4(u32x4 rs4, unsigned lds_addr, unsigned voffset) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                 :: "v"(voffset), "s"(rs4), "s"(lds_addr) : "memory", "m0");
+}
+
+// 16 B per lane into LDS in one of two forms.
 // COUNTED = false: the compiler's builtin; it then treats every later LDS read as dependent on the DMA and
 // drains vmcnt to 0 before each barrier.  COUNTED = true: the same instruction issued from inline assembly, which
 // leaves the vmcnt bookkeeping to the kernel (counted waits, two tiles in flight).  Loads complete in issue
@@ -82,9 +96,7 @@ template <bool COUNTED>
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, u32x4 rs4, unsigned char* lds, unsigned voffset) {
     if (COUNTED) {
         typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
-        const unsigned lds_addr = (unsigned)(unsigned long long)(lds_byte_ptr)lds;
-        asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                     :: "v"(voffset), "s"(rs4), "s"(lds_addr) : "memory", "m0");
+        dma_lds16(rs4, (unsigned)(unsigned long long)(lds_byte_ptr)lds, voffset);
     } else {
         typedef __attribute__((address_space(3))) void* lds_void_ptr;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_ptr)lds, 16, voffset, 0, 0, 0);

@@ -70,12 +70,6 @@ constexpr int GM = 8;                      // pixel tiles per group of the item 
 typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
-// one 1-KiB LDS-DMA piece: 16 B per lane from buffer offset `voff` to LDS address `lds_addr` + 16 * lane
-__device__ __forceinline__ void dma_piece(u32x4 rs4, unsigned lds_addr, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                 :: "v"(voff), "s"(rs4), "s"(lds_addr) : "memory", "m0");
-}
-
 struct WideArgs {
     int tiles_m, tiles_n, M, Kd;
     int splitk, nks;          // K steps per split (splitk == 1: nks = all)
@@ -178,8 +172,8 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(ConvArgs a, WideArgs 
 #define WG_PIECES(P, RS4, LDS, R, OFF0, OFF1)                                                     \
     {                                                                                             \
         const unsigned kb_ = (unsigned)P##_kt * (unsigned)ROWB, bo_ = P##_par * (unsigned)BUF_B;  \
-        dma_piece(RS4, LDS(R, 0) + bo_, P##OFF0 + kb_);                                           \
-        dma_piece(RS4, LDS(R, 1) + bo_, P##OFF1 + kb_);                                           \
+        dma_lds16(RS4, LDS(R, 0) + bo_, P##OFF0 + kb_);                                           \
+        dma_lds16(RS4, LDS(R, 1) + bo_, P##OFF1 + kb_);                                           \
     }
 #define WG_DMA_W0() WG_PIECES(c0, wrs4, WG_WLDS, 0, _w0, _w1)
 #define WG_DMA_X0() WG_PIECES(c0, xrs4, WG_XLDS, 0, _x0, _x1)

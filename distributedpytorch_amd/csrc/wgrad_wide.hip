@@ -52,11 +52,6 @@ constexpr int TILE_F = 256 * 256;          // floats per output tile
 typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
 typedef __attribute__((address_space(3))) short4v* lds_s4_ptr;
 
-__device__ __forceinline__ void dma_piece(u32x4 rs4, unsigned lds_addr, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                 :: "v"(voff), "s"(rs4), "s"(lds_addr) : "memory", "m0");
-}
-
 __device__ __forceinline__ bf16x8 tr_pair(const unsigned char* p) {
     const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(p));
     const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(p + 1024));     // token rows + 4: the next piece
@@ -178,14 +173,14 @@ __global__ __launch_bounds__(512, 2) void wgrad_wide_kernel(WwArgs) {
 #define WW_DMA_A(P, R)                                                                            \
     {                                                                                             \
         const unsigned bo_ = P##_par * (unsigned)BUF_B;                                           \
-        dma_piece(P##_ars, WW_ALDS(R, 0) + bo_, P##_a0);                                          \
-        dma_piece(P##_ars, WW_ALDS(R, 1) + bo_, P##_a1);                                          \
+        dma_lds16(P##_ars, WW_ALDS(R, 0) + bo_, P##_a0);                                          \
+        dma_lds16(P##_ars, WW_ALDS(R, 1) + bo_, P##_a1);                                          \
     }
 #define WW_DMA_B(P, R)                                                                            \
     {                                                                                             \
         const unsigned bo_ = P##_par * (unsigned)BUF_B;                                           \
-        dma_piece(P##_brs, WW_BLDS(R, 0) + bo_, P##_b0);                                          \
-        dma_piece(P##_brs, WW_BLDS(R, 1) + bo_, P##_b1);                                          \
+        dma_lds16(P##_brs, WW_BLDS(R, 0) + bo_, P##_b0);                                          \
+        dma_lds16(P##_brs, WW_BLDS(R, 1) + bo_, P##_b1);                                          \
     }
 #define WW_DMA_A0() WW_DMA_A(c0, 0)
 #define WW_DMA_B0() WW_DMA_B(c0, 0)
