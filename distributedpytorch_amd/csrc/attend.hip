@@ -12,7 +12,8 @@
 //     (one small kernel ahead): 64 tiles are tested at a time, one per lane, and the ballot is walked bit by bit.  Any
 //     numbering is right - ranges that overlap are visited and masked element by element -, sorted ones are fast.
 //   * Scores are kept in the exponent's base 2 throughout; tanh(x) = 1 - 2 r with r = 1 / (1 + e^{2x}), so that
-//     1 - tanh^2 = 4 r (1 - r) costs no second transcendental in the backward kernels.
+//     1 - tanh^2 = 4 r (1 - r) costs no second transcendental in the backward kernels.  Near x = 0 that difference cancels
+//     and leaves the score some 1.8e-7 of the cap off: caps past CAP_MOST take a build with a relative error instead.
 //   * delta comes from the same MFMA as dP (the diagonal of O dO^T): a row with one visible key has dP = delta bit for
 //     bit, and its dS is exactly zero as the formula says.  O enters it with what its rounding took away (kept by the
 //     forward in bf16, `rest`): where a few keys carry a row, dS is a small difference of dP and delta, and delta from the
@@ -39,6 +40,10 @@ using namespace attn;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MASKED = -2.0e30f;       // below every running maximum (which starts at NEG_BIG): exp2 gives 0 even in a row without keys
 constexpr int BQ = 128;                  // rows of a workgroup
+// The kernels' builds by cap: none, one up to CAP_MOST, a wider one (map_score).  At CAP_MOST the first form leaves a score 4.5e-5
+// off, a hundredth of what rounding P to bf16 does.
+constexpr int NO_CAP = 0, CAP = 1, WIDE_CAP = 2;
+constexpr float CAP_MOST = 256.f;
 
 struct DocRange { int lo, hi; };         // of 32 or more rows; padded rows count as -1
 
@@ -273,16 +278,34 @@ __device__ __forceinline__ void feed(Read read, Use use) {
 struct Frag3 { bf16x8 a, b, c; };
 struct Frag2 { bf16x8 a, b; };
 
-// Scores in base 2 from raw products.  `r` (cap only): 1 / (1 + e^{2x}), from which 1 - tanh^2 = 4 r (1 - r).
-struct ScoreMap { float c, k1, cap2; };       // scale log2 e;  2 scale log2 e / cap;  cap log2 e
-__device__ __forceinline__ ScoreMap score_map(const AttendArgs& a, bool cap) {
-    return {a.scale * LOG2E, cap ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E};
+// Scores in base 2 from raw products, and with a cap a quarter of 1 - tanh^2 in `f`.
+//   CAP       r = 1 / (1 + e^{2u}), u = x / cap: cap (1 - 2 r), f = r (1 - r).
+//   WIDE_CAP  relative accuracy wherever the score lies: below |u| = 0.4 the series of tanh(u) / u in u^2 (what is cut off is 4e-9),
+//             from there on the same exponential of -2 |u|, which leaves 3e-7 of a tanh >= 0.38.
+struct ScoreMap { float c, k1, cap2, k0; };   // scale log2 e;  2 scale log2 e / cap;  cap log2 e;  scale / cap
+__device__ __forceinline__ ScoreMap score_map(const AttendArgs& a, int cap) {
+    return {a.scale * LOG2E, cap ? 2.f * a.scale / a.softcap * LOG2E : 0.f, a.softcap * LOG2E, cap ? a.scale / a.softcap : 0.f};
 }
-template <bool CAP>
-__device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& r) {
-    if (CAP) {
-        r = __builtin_amdgcn_rcpf(1.f + fast_exp2(s * m.k1));
+template <int CAPPED>
+__device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& f) {
+    if (CAPPED == CAP) {
+        const float r = __builtin_amdgcn_rcpf(1.f + fast_exp2(s * m.k1));
+        f = fmaf(-r, r, r);
         return fmaf(r, -2.f * m.cap2, m.cap2);
+    }
+    if (CAPPED == WIDE_CAP) {
+        const float u = s * m.k0, w = u * u;
+        float p = 21844.f / 6081075.f;
+        p = fmaf(p, w, -1382.f / 155925.f);
+        p = fmaf(p, w, 62.f / 2835.f);
+        p = fmaf(p, w, -17.f / 315.f);
+        p = fmaf(p, w, 2.f / 15.f);
+        p = fmaf(p, w, -1.f / 3.f);
+        p = fmaf(p, w, 1.f);
+        const float t = u * p, e = fast_exp2(-fabsf(s * m.k1)), r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
+        const bool near = w < 0.16f;
+        f = near ? fmaf(-0.25f * t, t, 0.25f) : er * r;
+        return near ? s * m.c * p : copysignf(fmaf(er, -2.f * m.cap2, m.cap2), s);
     }
     return s * m.c;
 }
@@ -342,7 +365,7 @@ template <int DH> constexpr int stage_bytes() { return 2 * tile_bytes<DH>(); }
 template <int DH> constexpr int occupancy() { return DH == 64 ? 3 : 2; }
 
 // ------------------------------------------------------------------------------ forward
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAPPED, bool BIAS>
 __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(AttendArgs a, unsigned short* __restrict__ out, unsigned short* __restrict__ rest, float* __restrict__ lse2) {
     constexpr int KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB];
@@ -362,9 +385,9 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
     const int pre = seen_prefix(a, b);
     const int lim = max(qc, pre - 1);                               // the last key that this lane's query sees
     const int qdoc = docs != nullptr ? docs[qc] : 0;
-    const ScoreMap sm = score_map(a, CAP);
+    const ScoreMap sm = score_map(a, CAPPED);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-    const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
+    const BiasFrag bf(BIAS && !CAPPED ? a.slopes[head] / a.scale : 0.f, lane);
 
     TileWalk<false> walk;
     walk.open(docs != nullptr ? a.ranges + (long)b * tiles : nullptr, tiles, q0, wave, 0, (max(min(q0 + BQ, T), pre) + TILE - 1) / TILE);
@@ -414,18 +437,18 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         __builtin_amdgcn_s_setprio(0);
         // y = c S + add, in base 2: the scale and what is the same for a lane's whole tile ride the exponent's multiply-add
         float c = sm.c, add = 0.f;
-        if (BIAS && !CAP && (jt + TILE - 1 <= qw0 || pre <= qw0)) {  // wave-uniform: no visible key lies behind its query
+        if (BIAS && !CAPPED && (jt + TILE - 1 <= qw0 || pre <= qw0)) {  // wave-uniform: no visible key lies behind its query
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2) S[t2] = bf.add(S[t2], t2);
             add = slope2 * (float)(jt - q);
-        } else if (CAP || BIAS) {
+        } else if (CAPPED || BIAS) {
             c = 1.f;
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float rr;
-                    S[t2][r] = map_score<CAP>(sm, S[t2][r], rr);
+                    float f;
+                    S[t2][r] = map_score<CAPPED>(sm, S[t2][r], f);
                     if (BIAS) S[t2][r] = fmaf(-slope2, fabsf((float)(q - jt - 4 * h) - (float)(32 * t2 + acc_row(r, 0))), S[t2][r]);
                 }
         }
@@ -449,9 +472,9 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[t2][r]);
         mx = xhalf_max(mx);
-        const float peak = BIAS && !CAP ? fmaf(mx, c, add) : CAP ? mx : mx * c, mn = fmaxf(m, peak);
+        const float peak = BIAS && !CAPPED ? fmaf(mx, c, add) : CAPPED ? mx : mx * c, mn = fmaxf(m, peak);
         const bool grew = mn > m;
-        float off = BIAS && !CAP ? add - mn : -mn;
+        float off = BIAS && !CAPPED ? add - mn : -mn;
         if (!full) {
             off = peak >= m ? 0.f : peak - m;                       // (0 as such: the difference would be contracted)
 #pragma unroll
@@ -464,7 +487,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
         for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = fast_exp2(CAP ? S[t2][r] + off : fmaf(S[t2][r], c, off));
+                const float p = fast_exp2(CAPPED ? S[t2][r] + off : fmaf(S[t2][r], c, off));
                 S[t2][r] = p;
                 rsum += p;
             }
@@ -527,7 +550,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_fwd_kernel(Attend
 }
 
 // ------------------------------------------------------------------------------ dQ (query-stationary), and delta
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAPPED, bool BIAS>
 __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(AttendArgs a, const unsigned short* __restrict__ out, const unsigned short* __restrict__ rest,
                                                                             const unsigned short* __restrict__ dout, const float* __restrict__ lse2,
                                                                             float2* __restrict__ stats, unsigned short* __restrict__ dq) {
@@ -551,9 +574,9 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
     const int pre = seen_prefix(a, b);
     const int lim = max(qc, pre - 1);
     const int qdoc = docs != nullptr ? docs[qc] : 0;
-    const ScoreMap sm = score_map(a, CAP);
+    const ScoreMap sm = score_map(a, CAPPED);
     const float slope2 = BIAS ? a.slopes[head] * LOG2E : 0.f;
-    const BiasFrag bf(BIAS && !CAP ? a.slopes[head] / a.scale : 0.f, lane);
+    const BiasFrag bf(BIAS && !CAPPED ? a.slopes[head] / a.scale : 0.f, lane);
     const float lse_q = lse2[((long)b * a.Hq + head) * T + qc];
 
     TileWalk<false> walk;
@@ -623,10 +646,10 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
                             dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b, dof[kk], dP, 0, 0, 0);
                         });
             float c = sm.c, add = -lse_q;
-            if (BIAS && !CAP && (kt0 + 31 <= qw0 || pre <= qw0)) {  // as in the forward
+            if (BIAS && !CAPPED && (kt0 + 31 <= qw0 || pre <= qw0)) {  // as in the forward
                 S = bf.add(S, 0);
                 add += slope2 * (float)(kt0 - q);
-            } else if (BIAS && !CAP) {
+            } else if (BIAS && !CAPPED) {
                 c = 1.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -634,11 +657,10 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (CAP) {
-                    float rr;
-                    float e = map_score<CAP>(sm, S[r], rr);
+                if (CAPPED) {
+                    float f, e = map_score<CAPPED>(sm, S[r], f);
                     if (BIAS) e = fmaf(-slope2, fabsf((float)(q - kt0 - 4 * h) - (float)acc_row(r, 0)), e);
-                    S[r] = fast_exp2(e - lse_q) * (dP[r] - del) * fmaf(-rr, rr, rr);      // (1 - tanh^2) / 4; the rest behind the product
+                    S[r] = fast_exp2(e - lse_q) * (dP[r] - del) * f;                  // (1 - tanh^2) / 4; the rest behind the product
                 } else {
                     S[r] = fast_exp2(fmaf(S[r], c, add)) * (dP[r] - del);
                 }
@@ -654,7 +676,7 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
                             [&](int i, bf16x8 f) { dQt[i % DI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, dsb[i / DI], dQt[i % DI], 0, 0, 0); });
         }
     }
-    if (q < T) store_cols(dq + orow, dQt, qdoc >= 0 ? (CAP ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
+    if (q < T) store_cols(dq + orow, dQt, qdoc >= 0 ? (CAPPED ? 4.f : 1.f) * a.scale : 0.f, h, a.D);
 }
 
 // ------------------------------------------------------------------------------ dK / dV (key-stationary, no atomics)
@@ -665,10 +687,10 @@ __global__ __launch_bounds__(256, occupancy<DH>()) void attend_bwd_q_kernel(Atte
 // ld: the queries' (lse, delta) from row 4 h on; BIAS: lse + slope (i mod 64), so that -slope (i - j) - lse =
 // slope (j - jt) - ld.x where no query that sees a key lies in front of it (`linear`), and elsewhere the sign is put right
 // per element.  to_key: key - first query - 4 h; in_tile: key - first query of the 64-row tile.
-template <bool CAP, bool BIAS>
+template <int CAPPED, bool BIAS>
 __device__ __forceinline__ void key_side(floatx16& S, floatx16& dP, const float2* ld, const ScoreMap& sm, float slope2, bool linear, int to_key, int in_tile) {
     const float add = slope2 * (float)in_tile, behind = !BIAS || linear ? 0.f : 2.f * slope2;
-    if (BIAS && !CAP && !linear) {                                  // in raw units, in front of the scale
+    if (BIAS && !CAPPED && !linear) {                                  // in raw units, in front of the scale
         const float f = behind / sm.c;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = fmaf(-f, fmaxf((float)to_key - (float)acc_row(r, 0), 0.f), S[r]);
@@ -677,11 +699,11 @@ __device__ __forceinline__ void key_side(floatx16& S, floatx16& dP, const float2
     for (int r = 0; r < 16; ++r) {
         const int row = acc_row(r, 0);
         const float2 x = ld[row];
-        float rr, off = BIAS ? x.x - add : x.x;
-        if (BIAS && CAP) off = fmaf(behind, fmaxf((float)to_key - (float)row, 0.f), off);
-        S[r] = fast_exp2(CAP ? map_score<true>(sm, S[r], rr) - off : fmaf(S[r], sm.c, -off));
+        float f, off = BIAS ? x.x - add : x.x;
+        if (BIAS && CAPPED) off = fmaf(behind, fmaxf((float)to_key - (float)row, 0.f), off);
+        S[r] = fast_exp2(CAPPED ? map_score<CAPPED>(sm, S[r], f) - off : fmaf(S[r], sm.c, -off));
         dP[r] = S[r] * (dP[r] - x.y);
-        if (CAP) dP[r] *= fmaf(-rr, rr, rr);                        // (1 - tanh^2) / 4; the rest behind the product
+        if (CAPPED) dP[r] *= f;                                     // (1 - tanh^2) / 4; the rest behind the product
     }
 }
 
@@ -691,13 +713,13 @@ struct KvOut {
     float* part;                         // nullptr: whole groups
     int heads;                           // query heads of a workgroup
 };
-template <bool CAP, int DI>
+template <int CAPPED, int DI>
 __device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, const floatx16 (&dKt)[DI], const floatx16 (&dVt)[DI], int b, int key, int hq0,
                                           bool live, int h) {
     if (key >= a.T) return;
     const int group = a.Hq / a.Hkv;
     const long row = (((long)b * a.T + key) * a.Hkv + hq0 / group) * a.D;
-    const float kscale = live ? (CAP ? 4.f : 1.f) * a.scale : 0.f, vscale = live ? 1.f : 0.f;
+    const float kscale = live ? (CAPPED ? 4.f : 1.f) * a.scale : 0.f, vscale = live ? 1.f : 0.f;
     if (o.part == nullptr) {
         store_cols(o.dk + row, dKt, kscale, h, a.D);
         store_cols(o.dv + row, dVt, vscale, h, a.D);
@@ -717,7 +739,7 @@ __device__ __forceinline__ void store_key(const AttendArgs& a, const KvOut& o, c
         }
 }
 
-template <bool CAP, bool BIAS>
+template <int CAPPED, bool BIAS>
 __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, const unsigned short* __restrict__ dout,
                                                                const float2* __restrict__ stats, KvOut o) {
     constexpr int DH = 64, KK = DH / 16, DI = DH / 32, TB = tile_bytes<DH>(), SB = stage_bytes<DH>();
@@ -735,7 +757,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
     const int tiles = (T + TILE - 1) / TILE;
     const int pre = seen_prefix(a, b);
     const int kdoc = docs != nullptr ? docs[keyc] : 0;
-    const ScoreMap sm = score_map(a, CAP);
+    const ScoreMap sm = score_map(a, CAPPED);
 
     bf16x8 kf[KK], vf[KK];
     load_frags<DH>(kbase + (long)keyc * a.kt, h, a.D, kf);
@@ -800,7 +822,7 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
                 }
                 __builtin_amdgcn_s_setprio(0);
                 const float2* ld4 = lds_s + 32 * t2 + 4 * h;
-                key_side<CAP, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
+                key_side<CAPPED, BIAS>(S, dP, ld4, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - jt);
                 if (!full) {
                     unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
                     if (!same) bits &= doc_bits(Qd + 32 * t2, h, kdoc);
@@ -825,14 +847,14 @@ __global__ __launch_bounds__(256, 3) void attend_bwd_kv_kernel(AttendArgs a, con
         }
 #undef DPA_FETCH_Q
     }
-    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
+    store_key<CAPPED>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
 }
 
 // The same at width 128.  Two accumulators of 32 keys x 128 channels and both stationary operands are 192 registers; with what
 // two waves per SIMD leave beside them every fragment is read, waited for and used before the next one is read
 // (one row of 8192, 16 heads over 4: 634 us, the form below 500).  So the workgroup's values stay in LDS instead, 32 KiB, and are read as they are needed; to fit two workgroups
 // in a CU all the same, a stage is a half tile of 32 queries.
-template <bool CAP, bool BIAS>
+template <int CAPPED, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a, const unsigned short* __restrict__ dout, const float2* __restrict__ stats, KvOut o) {
     constexpr int DH = 128, ROWS = 32, KK = DH / 16, DI = DH / 32, TB = ROWS * DH * 2, SB = 2 * TB;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SB + BQ * DH * 2];   // two stages of queries and output gradients, then the values
@@ -854,7 +876,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a
     const int* docs = a.docs != nullptr ? a.docs + (long)b * T : nullptr;
     const int pre = seen_prefix(a, b);
     const int kdoc = docs != nullptr ? docs[keyc] : 0;
-    const ScoreMap sm = score_map(a, CAP);
+    const ScoreMap sm = score_map(a, CAPPED);
     zero_unless<DH>(kdoc >= 0, kf);                                 // (a padded key's values reach its own column of dP only, which its mask zeroes)
     floatx16 dKt[DI], dVt[DI];
 #pragma unroll
@@ -901,7 +923,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a
                             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a, kf[kk], S, 0, 0, 0);
                             dP = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b, f.c, dP, 0, 0, 0);
                         });
-            key_side<CAP, BIAS>(S, dP, lds_ss[stage] + 4 * h, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - qt0 / TILE * TILE);
+            key_side<CAPPED, BIAS>(S, dP, lds_ss[stage] + 4 * h, sm, slope2, qt0 >= kw0 + 31 || pre <= qt0, key - qt0 - 4 * h, key - qt0 / TILE * TILE);
             if (!full) {
                 unsigned bits = range_bits(key_from - qt0 - 4 * h, T - qt0 - 4 * h);
                 if (!same) bits &= doc_bits(Qds[stage], h, kdoc);
@@ -920,7 +942,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a
         }
 #undef DPA_FETCH_Q
     }
-    store_key<CAP>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
+    store_key<CAPPED>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
 }
 
 // dk, dv [n] = the sum of their parts [parts][2][n] in order, rounded once (n a multiple of 8)
@@ -937,20 +959,20 @@ __global__ __launch_bounds__(256) void fold_parts_kernel(const float* __restrict
     }
 }
 
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAPPED, bool BIAS>
 void fwd_of(const AttendArgs& a, void* out, void* rest, float* lse2, hipStream_t st) {
-    hipLaunchKernelGGL((attend_fwd_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, (a.T + BQ - 1) / BQ), dim3(256), 0, st, a, (unsigned short*)out,
+    hipLaunchKernelGGL((attend_fwd_kernel<DH, CAPPED, BIAS>), dim3(a.Hq, a.B, (a.T + BQ - 1) / BQ), dim3(256), 0, st, a, (unsigned short*)out,
                        (unsigned short*)rest, lse2);
 }
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAPPED, bool BIAS>
 void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* dout, const float* lse2, void* stats, void* dq, void* dk, void* dv,
             float* part, hipStream_t st) {
     const int blocks = (a.T + BQ - 1) / BQ;
-    hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAP, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
+    hipLaunchKernelGGL((attend_bwd_q_kernel<DH, CAPPED, BIAS>), dim3(a.Hq, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)out,
                        (const unsigned short*)rest, (const unsigned short*)dout, lse2, (float2*)stats, (unsigned short*)dq);
     const int parts = part != nullptr ? attend_kv_parts(a) : 1, heads = a.Hq / a.Hkv / parts;
     const KvOut o{(unsigned short*)dk, (unsigned short*)dv, part, heads};
-    constexpr auto kv = DH == 64 ? attend_bwd_kv_kernel<CAP, BIAS> : attend_bwd_kv_wide_kernel<CAP, BIAS>;
+    constexpr auto kv = DH == 64 ? attend_bwd_kv_kernel<CAPPED, BIAS> : attend_bwd_kv_wide_kernel<CAPPED, BIAS>;
     hipLaunchKernelGGL(kv, dim3(a.Hkv * parts, a.B, blocks), dim3(256), 0, st, a, (const unsigned short*)dout, (const float2*)stats, o);
     if (part != nullptr) {
         const long n = (long)a.B * a.T * a.Hkv * a.D, grid = (2 * n / 8 + 255) / 256;
@@ -961,16 +983,19 @@ void bwd_of(const AttendArgs& a, const void* out, const void* rest, const void* 
 }  // namespace
 
 // one build per (width, cap, bias): the masks are wave-uniform branches inside
+#define DPA_ATTEND_BIAS(F, DH_, CAP_, ...)                                                                              \
+    do {                                                                                                                \
+        if (a.slopes != nullptr) F<DH_, CAP_, true>(__VA_ARGS__); else F<DH_, CAP_, false>(__VA_ARGS__);                \
+    } while (0)
+#define DPA_ATTEND_CAP(F, DH_, ...)                                                                                     \
+    do {                                                                                                                \
+        if (!(a.softcap > 0.f)) DPA_ATTEND_BIAS(F, DH_, NO_CAP, __VA_ARGS__);                                           \
+        else if (a.softcap <= CAP_MOST) DPA_ATTEND_BIAS(F, DH_, CAP, __VA_ARGS__);                                      \
+        else DPA_ATTEND_BIAS(F, DH_, WIDE_CAP, __VA_ARGS__);                                                            \
+    } while (0)
 #define DPA_ATTEND_PICK(F, ...)                                                                                         \
     do {                                                                                                                \
-        const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;                                                   \
-        if (a.D <= 64) {                                                                                                \
-            if (cap) { if (bias) F<64, true, true>(__VA_ARGS__); else F<64, true, false>(__VA_ARGS__); }                \
-            else { if (bias) F<64, false, true>(__VA_ARGS__); else F<64, false, false>(__VA_ARGS__); }                  \
-        } else {                                                                                                        \
-            if (cap) { if (bias) F<128, true, true>(__VA_ARGS__); else F<128, true, false>(__VA_ARGS__); }              \
-            else { if (bias) F<128, false, true>(__VA_ARGS__); else F<128, false, false>(__VA_ARGS__); }                \
-        }                                                                                                               \
+        if (a.D <= 64) DPA_ATTEND_CAP(F, 64, __VA_ARGS__); else DPA_ATTEND_CAP(F, 128, __VA_ARGS__);                    \
     } while (0)
 
 void attend_doc_ranges(const int* docs, void* ranges, int B, int T, hipStream_t st) {

@@ -59,7 +59,7 @@ dpa::AttendArgs attend_args(const Tensor& q, const Tensor& k, const Tensor& v, b
     TORCH_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && D >= 8 && D % 8 == 0 && D <= 128, "attend: heads");
     TORCH_CHECK(B <= 65535 && T <= (1 << 22) && Hq <= 65535 && (int64_t)Hq * D < (1 << 23), "attend: oversized problem");
     for (const Tensor* t : {&q, &k, &v}) TORCH_CHECK(T <= 1 || t->stride(1) < (1 << 23), "attend: token stride");
-    TORCH_CHECK(scale > 1e-12 && scale < 1e12 && softcap >= 0.0 && softcap < 1e12, "attend: scale, softcap");
+    TORCH_CHECK(scale > 1e-12 && scale < 1e12 && (softcap == 0.0 || (softcap > 1e-12 && softcap < 1e12)), "attend: scale, softcap");
     dpa::AttendArgs a{};
     a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
     a.qb = row_stride(q, 0); a.qt = row_stride(q, 1); a.qh = row_stride(q, 2);

@@ -55,7 +55,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     in place.  On the GPU: bf16, ``D`` a multiple of 8 up to 128.
 
     Score of query ``i`` and key ``j``: ``x = scale * q_i . k_j`` (``scale`` defaults to ``D ** -0.5``), then
-    ``softcap * tanh(x / softcap)`` if ``softcap > 0``, then ``x - slopes[h] * |i - j|`` (``slopes [Hq]``, fp32).
+    ``softcap * tanh(x / softcap)`` if ``softcap`` is not 0 (from 1e-12 to 1e12), then ``x - slopes[h] * |i - j|`` (``slopes [Hq]``, fp32).
     Visible: ``j <= i``, or ``j < prefix[b]`` (``prefix [B]``, int32, clamped to ``0 .. T``), or every ``j`` with
     ``causal=False``; and, with ``documents [B,T]`` (int32, any numbering, sorted ones run fastest), only keys of the query's
     own document.  A token with a negative document number is padding: it sees nothing, is seen by nothing, its output and
@@ -83,8 +83,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     softcap = float(softcap)
     if not 1e-12 < scale < 1e12:
         raise ValueError(f"attention: scale must be positive and finite, got {scale}")
-    if not 0.0 <= softcap < 1e12:
-        raise ValueError(f"attention: softcap must be 0 (none) or positive and finite, got {softcap}")
+    if softcap != 0.0 and not 1e-12 < softcap < 1e12:
+        raise ValueError(f"attention: softcap must be 0 (none) or between 1e-12 and 1e12, got {softcap}")
     for name, t, shape, dtype in (("slopes", slopes, (Hq,), torch.float32), ("documents", documents, (B, T), torch.int32),
                                   ("prefix", prefix, (B,), torch.int32)):
         if t is None:

@@ -143,6 +143,20 @@ def test_attention_forward_and_backward(case):
         assert torch.equal(ops.attention(*leaf, **_on(kw)), out)                   # alone, and the same bits again
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("softcap,gain,slopes", [(255.0, 2.0, False), (257.0, 2.0, True), (1e3, 2.0, False), (1e5, 2.0, True), (1e7, 2.0, False), (1e11, 2.0, True),
+                                                 (300.0, 10.0, False), (2000.0, 10.0, False)])
+def test_attention_caps_far_from_the_scores(softcap, gain, slopes, D):
+    """Caps up to 256 leave a score 2e-7 of the cap off, wider ones 3e-7 of the score itself; raw scores of deviation gain^2 are off by
+    another 2^-23 of their size, and none here is past 700: together below the 2^-12 of P that the bounds count."""
+    q, k, v, do, kw = _attend_inputs(1, 200, 4, 2, D, dict(softcap=softcap, gain=gain, slopes=slopes))
+    ref = _attend_ref(q, k, v, do, **kw)
+    leaf = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaf, **_on(kw))
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaf, do.to(DEV)))):
+        _within(got, *ref[name], name)
+
+
 def test_attention_reads_strided_views_in_place():
     B, T, Hq, Hkv, D = 2, 150, 4, 2, 64
     pack = _rand(B, T, Hq + 2 * Hkv, D, seed=5).to(DEV)

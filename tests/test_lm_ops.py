@@ -101,6 +101,14 @@ def test_attention_refusals():
         ops.attention(q.long(), k.long(), k.long())
 
 
+def test_attention_cap_outside_its_range():
+    """A cap that fp32 cannot hold would be no cap at all on the GPU."""
+    q = torch.zeros(1, 2, 1, 8)
+    for softcap in (1e-46, 1e-13, 1e12, math.inf):
+        with pytest.raises(ValueError):
+            ops.attention(q, q, q, softcap=softcap)
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("R", [0, 4, 8])
 @pytest.mark.parametrize("norm", [False, True])
