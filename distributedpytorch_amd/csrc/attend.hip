@@ -12,7 +12,7 @@
 //     (one small kernel ahead): 64 tiles are tested at a time, one per lane, and the ballot is walked bit by bit.  Any
 //     numbering is right - ranges that overlap are visited and masked element by element -, sorted ones are fast.
 //   * Scores are kept in the exponent's base 2 throughout; tanh(x) = 1 - 2 r with r = 1 / (1 + e^{2x}), so that
-//     1 - tanh^2 = 4 r (1 - r) costs no second transcendental in the backward kernels.  Near x = 0 that difference cancels
+//     1 - tanh^2 = 4 r (e^{2x} r) costs no second transcendental in the backward kernels.  Near x = 0 that difference cancels
 //     and leaves the score some 1.8e-7 of the cap off: caps past CAP_MOST take a build with a relative error instead.
 //   * delta comes from the same MFMA as dP (the diagonal of O dO^T): a row with one visible key has dP = delta bit for
 //     bit, and its dS is exactly zero as the formula says.  O enters it with what its rounding took away (kept by the
@@ -279,7 +279,8 @@ struct Frag3 { bf16x8 a, b, c; };
 struct Frag2 { bf16x8 a, b; };
 
 // Scores in base 2 from raw products, and with a cap a quarter of 1 - tanh^2 in `f`.
-//   CAP       r = 1 / (1 + e^{2u}), u = x / cap: cap (1 - 2 r), f = r (1 - r).
+//   CAP       r = 1 / (1 + e^{2u}), u = x / cap: cap (1 - 2 r), f = r (1 - r) with 1 - r as e^{2u} r: the difference itself has
+//             nothing left where u < -8, and there f is all the gradient that a row of such scores has.
 //   WIDE_CAP  relative accuracy wherever the score lies: below |u| = 0.4 the series of tanh(u) / u in u^2 (what is cut off is 4e-9),
 //             from there on the same exponential of -2 |u|, which leaves 3e-7 of a tanh >= 0.38.
 struct ScoreMap { float c, k1, cap2, k0; };   // scale log2 e;  2 scale log2 e / cap;  cap log2 e;  scale / cap
@@ -289,8 +290,8 @@ __device__ __forceinline__ ScoreMap score_map(const AttendArgs& a, int cap) {
 template <int CAPPED>
 __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& f) {
     if (CAPPED == CAP) {
-        const float r = __builtin_amdgcn_rcpf(1.f + fast_exp2(s * m.k1));
-        f = fmaf(-r, r, r);
+        const float e = fast_exp2(s * m.k1), r = __builtin_amdgcn_rcpf(1.f + e);
+        f = r * fminf(e * r, 1.f);                                  // (an infinite e: r = 0, and the NaN gives way to 1)
         return fmaf(r, -2.f * m.cap2, m.cap2);
     }
     if (CAPPED == WIDE_CAP) {

@@ -157,6 +157,24 @@ def test_attention_caps_far_from_the_scores(softcap, gain, slopes, D):
         _within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("softcap,sign", [(2.0, -1), (2.0, 1), (0.5, -1), (1e-11, -1), (1e-11, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_scores_all_at_one_end_of_the_cap(D, softcap, sign):
+    """Raw scores around 8 caps of one sign (but for the two smallest caps, where they lie past any exponential): 1 - tanh^2 is some
+    1e-7 of 1 and all that the scores' gradients are made of.  Each raw score is within 2^-22 of its size, 8 caps, so 1 - tanh^2 within
+    16 2^-22: inside the 2^-12 that the bounds count."""
+    B, T, H = 1, 140, 2
+    mean = math.sqrt(8 * min(max(softcap, 0.5), 2.0) / math.sqrt(D))
+    q, k = ((mean * (1 + 0.1 * _rand(B, T, H, D, seed=s, dtype=torch.float32))).to(torch.bfloat16) for s in (1, 2))
+    k = k * sign
+    v, do = (_rand(B, T, H, D, seed=s) for s in (3, 4))
+    ref = _attend_ref(q, k, v, do, softcap=softcap)
+    leaf = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaf, softcap=softcap)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaf, do.to(DEV)))):
+        _within(got, *ref[name], name)
+
+
 def test_attention_reads_strided_views_in_place():
     B, T, Hq, Hkv, D = 2, 150, 4, 2, 64
     pack = _rand(B, T, Hq + 2 * Hkv, D, seed=5).to(DEV)
