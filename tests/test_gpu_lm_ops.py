@@ -348,6 +348,26 @@ def test_heads_without_eps(Hq, Hkv, D):
     assert torch.equal(got[0].view(1, T, -1, D)[:, :, Hq + Hkv:].cpu(), gs[2])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_heads_value_gradients_stay_out_of_the_key_gain(bad, interleaved):
+    """Whatever the values' gradients hold reaches the projection's gradient alone, where it stands."""
+    Hq, Hkv, D = 3, 2, 64
+    x = _rand(2, 9, (Hq + 2 * Hkv) * D, seed=1).to(DEV).requires_grad_()
+    w = [(1 + 0.3 * _rand(D, seed=2 + i, dtype=torch.float32)).to(DEV).requires_grad_() for i in range(2)]
+    gs = [_rand(2, 9, h, D, seed=4 + i).to(DEV) for i, h in enumerate((Hq, Hkv, Hkv))]
+    f = ops.rotary_frequencies(D, device=DEV)
+
+    def grads():
+        return torch.autograd.grad(ops.qk_norm_rotary(x, Hq, Hkv, q_weight=w[0], k_weight=w[1], inv_freq=f, interleaved=interleaved), (x, *w), gs)
+    want = grads()
+    gs[2][1, 4, 1, 7] = bad
+    dx, dqw, dkw = grads()
+    assert torch.equal(dqw, want[1]) and torch.equal(dkw, want[2])
+    want[0].view(2, 9, -1, D)[1, 4, Hq + Hkv + 1, 7] = bad
+    assert torch.equal(dx.nan_to_num(nan=1e30), want[0].nan_to_num(nan=1e30))
+
+
 def test_heads_empty():
     w = torch.ones(16, device=DEV, requires_grad=True)
     x = torch.zeros(2, 0, 48, dtype=torch.bfloat16, device=DEV, requires_grad=True)
