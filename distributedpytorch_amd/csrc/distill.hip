@@ -240,14 +240,19 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
             });
         }
         const float2 mm = fold2<NW, true>(m, tm, red[0]);
-        const float m2 = mm.x * c;
+        // Exponents are differences from the maximum, and the sum divides: with the sum's logarithm added to the maximum instead, q
+        // would be half a place of the maximum off (fp32 logits around 1000: 4e-5 of q, 1e-7 so).  Where one multiply-add forms them,
+        // what m2's rounding takes moves all of a row's exponents alike and leaves with the sum; a row that is read again has its sum
+        // by parts from other maxima, so there the difference comes first (for every build: 851 instead of 808 us at 16,384 x 50,257).
+        const float mx = mm.x, m2 = mx * c;
+        const auto exponent = [&](float v) { return NREG > 0 ? fmaf(v, c, -m2) : (v - mx) * c; };
         if (NREG > 0)
             sweep([&](int, float (&v)[N], bool) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) s += fast_exp2(fmaf(v[j], c, -m2));
+                for (int j = 0; j < N; ++j) s += fast_exp2(exponent(v[j]));
             });
         else
-            s *= fast_exp2((m - mm.x) * c);
+            s *= fast_exp2((m - mx) * c);
         float x[KE], ts = 0.f;
 #pragma unroll
         for (int i = 0; i < KE; ++i) {
@@ -256,23 +261,23 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         }
         const float2 ss = fold2<NW, false>(s, ts, red[1]);
         const bool any = __syncthreads_or(live);                               // a row without a teacher gives nothing, whatever it holds
-        const float lse2 = m2 + log2f(ss.x);
+        const float inv = 1.f / ss.x, lsum = log2f(ss.x);
         float p[KE], term = 0.f;
 #pragma unroll
         for (int i = 0; i < KE; ++i) {
             const int k = tid + i * NT;
             p[i] = te.id[i] >= 0 ? expf(x[i]) / ss.y : 0.f;
             if (k < a.K) { ids_s[k] = te.id[i]; p_s[k] = p[i]; }
-            const float y = fmaf(te.z[i], c, -lse2);                           // log2 q
+            const float y = exponent(te.z[i]) - lsum;                          // log2 q
             if (te.id[i] >= 0) term += p[i] == 0.f ? 0.f : p[i] * (x[i] - logf(ss.y) - y * LN2);
         }
         if (next < a.N) load_student((const T*)a.logits + next * a.ld, nte);
         if (r.d != nullptr) {
-            const float g = a.grad_scale;
+            const float g = a.grad_scale * inv;
             if (any)
                 sweep([&](int i, float (&v)[N], bool sure) {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) v[j] = fast_exp2(fmaf(v[j], c, -lse2)) * g;
+                    for (int j = 0; j < N; ++j) v[j] = fast_exp2(exponent(v[j])) * g;
                     r.template store<WHOLE>(i, v, sure);
                 });
             else
@@ -288,7 +293,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
                 if (te.id[i] >= 0) {
                     float same = 0.f;
                     for (int k = 0; k < a.K; ++k) same += ids_s[k] == te.id[i] ? p_s[k] : 0.f;
-                    put1(r.d + te.id[i], (fast_exp2(fmaf(te.z[i], c, -lse2)) - same) * a.grad_scale);
+                    put1(r.d + te.id[i], (fast_exp2(exponent(te.z[i])) * inv - same) * a.grad_scale);
                 }
         if (any) total += term;
         __syncthreads();                                                       // ids_s and p_s are read

@@ -542,6 +542,28 @@ def test_distillation_forward_and_backward(case, ids32):
     assert torch.equal(z[:, :V], zd.detach().cpu()[:, :V])
 
 
+@pytest.mark.parametrize("V", [700, 5000, 33000, 110000])
+def test_distillation_does_not_feel_a_rows_offset(V):
+    """Logits of deviation 2 around 30,000 and -30,000: what is left of each class counts from the row's maximum, so the bounds are those
+    of the zero-mean rows (an exponent |y| < 100 off by 2^-24 relative), in all four builds."""
+    N, K, tau = 4, 20, 1.5
+    z = _rand(N, V, seed=V, std=2.0, dtype=torch.float32) + torch.tensor([0.0, 3e4, -3e4, 1e3])[:, None]
+    ids, t = _teacher(N, V, K, V)
+    live = (ids >= 0) & (ids < V) & (t > -math.inf)
+    at = torch.where(live, ids, 0)
+    logq = torch.log_softmax(z.double() / tau, 1)
+    logp = torch.log_softmax((t.double() / tau).masked_fill(~live, -math.inf), 1)
+    p, lq = logp.exp() * live, logq.gather(1, at)
+    loss = tau * tau * torch.where(live, p * (logp - lq), 0.0).sum() / N
+    size = tau * tau * torch.where(live, p * (logp.abs() + lq.abs() + 1), 0.0).sum() / N
+    full = torch.zeros(N, V, dtype=torch.float64).scatter_add_(1, at, p)
+    d = (logq.exp() - full) * tau / N
+    zd = z.to(DEV).requires_grad_()
+    got = ops.distillation_loss(zd, ids.to(DEV), t.to(DEV), temperature=tau)
+    _within(got, loss, 2.0 ** -16 * size, "loss")
+    _within(torch.autograd.grad(got, zd)[0], d, 2.0 ** -16 * (logq.exp() + full) * tau / N + U32 * d.abs() + 1e-38, "dlogits")
+
+
 def test_distillation_gradient_against_differences():
     N, V, K, tau = 6, 300, 12, 2.0
     z = _rand(N, V, seed=3, std=2.0, dtype=torch.float32).to(DEV).requires_grad_()
