@@ -27,7 +27,7 @@ namespace dpa {
 namespace {
 
 constexpr int KMAX = 1024;
-constexpr float NEG_BIG = -1.0e30f, LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOWEST = -3.4028234664e38f, LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float get1(const unsigned short* p) { return bf16_to_float(*p); }
 __device__ __forceinline__ float get1(const float* p) { return *p; }
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
             }
         };
         // maxima of the row and of the teacher's live entries (a NaN entry is live: the row's sums become NaN)
-        float m = NEG_BIG, s = 0.f, tm = -INFINITY;
+        float m = LOWEST, s = 0.f, tm = -INFINITY;
         bool live = false;
 #pragma unroll
         for (int i = 0; i < KE; ++i)
@@ -242,14 +242,24 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         const float2 mm = fold2<NW, true>(m, tm, red[0]);
         // Exponents are differences from the maximum, and the sum divides: with the sum's logarithm added to the maximum instead, q
         // would be half a place of the maximum off (fp32 logits around 1000: 4e-5 of q, 1e-7 so).  Where one multiply-add forms them,
-        // what m2's rounding takes moves all of a row's exponents alike and leaves with the sum; a row that is read again has its sum
-        // by parts from other maxima, so there the difference comes first (for every build: 851 instead of 808 us at 16,384 x 50,257).
+        // what m2's rounding takes moves all of a row's exponents alike and leaves with the sum - as long as it is small: rows that are far
+        // from zero (masked as a whole with the type's lowest value, say) have the difference formed first, and so has a row that is
+        // read again, whose sum is made by parts from other maxima.  (For every row: 851 instead of 808 us at 16,384 x 50,257.)
         const float mx = mm.x, m2 = mx * c;
-        const auto exponent = [&](float v) { return NREG > 0 ? fmaf(v, c, -m2) : (v - mx) * c; };
+        const bool far = NREG == 0 || !(fabsf(m2) < 1e6f);                     // the same for the whole workgroup
+        const auto near_exponent = [&](float v) { return fmaf(v, c, -m2); };
+        const auto far_exponent = [&](float v) { return (v - mx) * c; };
+        const auto exponent = [&](float v) { return far ? far_exponent(v) : near_exponent(v); };
+        const auto with_exponent = [&](auto&& body) {                          // not chosen element by element
+            if (far) body(far_exponent);
+            else body(near_exponent);
+        };
         if (NREG > 0)
-            sweep([&](int, float (&v)[N], bool) {
+            with_exponent([&](auto&& e) {
+                sweep([&](int, float (&v)[N], bool) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) s += fast_exp2(exponent(v[j]));
+                    for (int j = 0; j < N; ++j) s += fast_exp2(e(v[j]));
+                });
             });
         else
             s *= fast_exp2((m - mx) * c);
@@ -275,10 +285,12 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         if (r.d != nullptr) {
             const float g = a.grad_scale * inv;
             if (any)
-                sweep([&](int i, float (&v)[N], bool sure) {
+                with_exponent([&](auto&& e) {
+                    sweep([&](int i, float (&v)[N], bool sure) {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) v[j] = fast_exp2(exponent(v[j])) * g;
-                    r.template store<WHOLE>(i, v, sure);
+                        for (int j = 0; j < N; ++j) v[j] = fast_exp2(e(v[j])) * g;
+                        r.template store<WHOLE>(i, v, sure);
+                    });
                 });
             else
                 for (int i = tid; i < nv; i += NT) {

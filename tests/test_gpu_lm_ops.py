@@ -564,6 +564,35 @@ def test_distillation_does_not_feel_a_rows_offset(V):
     _within(torch.autograd.grad(got, zd)[0], d, 2.0 ** -16 * (logq.exp() + full) * tau / N + U32 * d.abs() + 1e-38, "dlogits")
 
 
+@pytest.mark.parametrize("V", [40, 700, 5000, 33000, 110000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distillation_rows_of_the_lowest_values(V, dtype):
+    """Rows whose classes all hold the type's lowest value, or numbers far below any others, are rows like any: a row of one value is
+    uniform, and one of two values far apart is uniform over the higher ones.  q is then a quotient of exact numbers: bounds as for any
+    row.  Masked places in an ordinary row are zeros."""
+    low = torch.finfo(dtype).min
+    z = torch.empty(6, V, dtype=dtype)
+    z[0], z[1], z[2], z[3] = low, -2e30, 1e37, low
+    z[3, ::4] = -1e35
+    z[4] = _rand(V, seed=V, dtype=dtype)
+    z[4, 1::3] = low
+    z[5] = low
+    z[5, 1] = 3.0
+    ids = torch.tensor([[0, 4], [4, 8], [8, 12], [0, 16], [0, 6], [1, 1]])
+    t = torch.tensor([[0.5, -0.5]]).repeat(6, 1)
+    logq = torch.log_softmax(z.double(), 1)
+    logp = torch.log_softmax(t.double(), 1)
+    p, lq = logp.exp(), logq.gather(1, ids)
+    loss = (p * (logp - lq)).sum() / 6
+    size = (p * (logp.abs() + lq.abs() + 1)).sum() / 6
+    full = torch.zeros(6, V, dtype=torch.float64).scatter_add_(1, ids, p)
+    d = (logq.exp() - full) / 6
+    zd = z.to(DEV).requires_grad_()
+    got = ops.distillation_loss(zd, ids.to(DEV), t.to(DEV))
+    _within(got, loss, 2.0 ** -16 * size, "loss")
+    _within(torch.autograd.grad(got, zd)[0], d, 2.0 ** -16 * (logq.exp() + full) / 6 + (U16 if dtype == torch.bfloat16 else U32) * d.abs() + 1e-38, "dlogits")
+
+
 def test_distillation_gradient_against_differences():
     N, V, K, tau = 6, 300, 12, 2.0
     z = _rand(N, V, seed=3, std=2.0, dtype=torch.float32).to(DEV).requires_grad_()
