@@ -21,6 +21,7 @@ def _plain(logits, ids, teacher, n_classes, tau):
     live = (ids >= 0) & (ids < n_classes) & (teacher != -math.inf)
     rows = live.any(1)
     z = torch.where(rows[:, None], z, 0.0)               # a row without a teacher gives nothing, whatever it holds
+    z = z - z.detach().amax(1, keepdim=True)             # what all classes share would cost the rest its digits
     lse = torch.logsumexp(z, 1, keepdim=True)
     t = (teacher.to(wide) / tau).masked_fill(~live, -math.inf).masked_fill(~rows[:, None], 0.0)
     logp = torch.log_softmax(t, 1)

@@ -218,6 +218,21 @@ def test_distillation_plain_path_against_loops_and_differences(tau):
     assert torch.equal(three, loss)
 
 
+def test_distillation_plain_path_does_not_feel_a_rows_offset():
+    """fp32 logits around 30,000, where one place is 2^-9, and rows of the lowest value: each term within some places of its own size."""
+    z = torch.randn(4, 50, generator=_g(1)) + torch.tensor([0.0, 3e4, -3e4, 0.0])[:, None]
+    z[3] = torch.finfo(torch.float32).min
+    ids, t = torch.arange(12).view(4, 3), torch.randn(4, 3, generator=_g(2))
+    a, b = z.clone().requires_grad_(), z.double().requires_grad_()
+    one, two = ops.distillation_loss(a, ids, t), ops.distillation_loss(b, ids, t.double())
+    q, p = torch.softmax(z.double(), 1), torch.softmax(t.double(), 1)
+    by_hand = (p * (p.log() - q.log().gather(1, ids))).sum() / 4
+    assert abs(two.item() - by_hand.item()) < 1e-12
+    assert abs(one.item() - by_hand.item()) < 1e-5
+    da, db = torch.autograd.grad(one, a)[0], torch.autograd.grad(two, b)[0]
+    torch.testing.assert_close(da.double(), db, rtol=0, atol=1e-6)
+
+
 def test_distillation_refusals():
     z, ids, t = torch.zeros(4, 10), torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
     ops.distillation_loss(z, ids, t)
