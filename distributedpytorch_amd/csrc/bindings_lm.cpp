@@ -302,12 +302,12 @@ struct EmbedNode : public torch::autograd::Function<EmbedNode> {
 Tensor token_embedding(const Tensor& tok, const Tensor& w, const Tensor& w_lp, double scale) { return EmbedNode::apply(tok, w, w_lp, scale); }
 
 // ---------------------------------------------------------------- distillation
-// -> loss [1], and the logits' gradient for an upstream gradient of 1 (undefined unless asked for)
-std::vector<Tensor> distill(const Tensor& logits_, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool want_grad) {
-    CHECK_ON(logits_, logits_); TORCH_CHECK(logits_.dim() == 2, "distill: logits [N, ld]");
-    const Tensor logits = flat16(logits_);                                     // rows lie on 16 bytes as those of the gradient do
+// ids and teacher's entries per row, the classes and the temperature as the kernel takes them; logits contiguous, on 16 bytes
+dpa::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau) {
+    TORCH_CHECK(logits.dim() == 2, "distill: logits [N, ld]");
     const bool bf = logits.scalar_type() == at::kBFloat16;
     TORCH_CHECK(bf || logits.scalar_type() == at::kFloat, "distill: logits must be bf16 or fp32");
+    CHECK_FLAT16(logits, logits, logits.scalar_type());
     CHECK_ON(ids, logits); TORCH_CHECK(ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt), "distill: ids int64 or int32");
     CHECK_FLAT(teacher, logits, at::kFloat);
     const int64_t N = logits.size(0), ld = logits.size(1);
@@ -315,32 +315,49 @@ std::vector<Tensor> distill(const Tensor& logits_, const Tensor& ids, const Tens
     const int64_t K = ids.size(1);
     TORCH_CHECK(K >= 1 && K <= dpa::distill_max_entries() && V >= 1 && V <= ld && ld < (1 << 30) && N < (1ll << 31), "distill: sizes");
     TORCH_CHECK(tau > 0.0, "distill: temperature");
-    Guard guard(logits.device());
-    const auto fopt = logits.options().dtype(at::kFloat);
-    Tensor loss = torch::empty({1}, fopt), rows = torch::empty({dpa::distill_blocks(bf, N, ld)}, fopt), d;
-    if (want_grad) d = torch::empty_like(logits);
     dpa::DistillArgs a{};
-    a.logits = logits.data_ptr(); a.dlogits = want_grad ? d.data_ptr() : nullptr;
-    a.ids = ids.data_ptr(); a.teacher = teacher.data_ptr<float>(); a.row_loss = rows.data_ptr<float>();
+    a.logits = logits.data_ptr(); a.ids = ids.data_ptr(); a.teacher = teacher.data_ptr<float>();
     a.N = N; a.ld = ld; a.V = (int)V; a.K = (int)K; a.ids64 = ids.scalar_type() == at::kLong;
     a.inv_tau = (float)(1.0 / tau);
-    const double n = N > 0 ? (double)N : 1.0;
-    a.grad_scale = (float)(tau / n);
+    a.grad_scale = (float)(tau / (N > 0 ? (double)N : 1.0));
+    return a;
+}
+
+// -> loss [1], and the logits' gradient for an upstream gradient of 1 (undefined unless asked for)
+std::vector<Tensor> distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool want_grad) {
+    dpa::DistillArgs a = distill_args(logits, ids, teacher, V, tau);
+    const bool bf = logits.scalar_type() == at::kBFloat16;
+    Guard guard(logits.device());
+    const auto fopt = logits.options().dtype(at::kFloat);
+    Tensor loss = torch::empty({1}, fopt), rows = torch::empty({dpa::distill_blocks(bf, a.N, a.ld)}, fopt), d;
+    if (want_grad) d = torch::empty_like(logits);
+    a.dlogits = want_grad ? d.data_ptr() : nullptr;
+    a.row_loss = rows.data_ptr<float>();
+    const double n = a.N > 0 ? (double)a.N : 1.0;
     dpa::distill(a, bf, (float)(tau * tau / n), loss.data_ptr<float>(), cur_stream());
     return {loss, d};
 }
 
-void scale_grad(Tensor& d, const Tensor& g) {
-    TORCH_CHECK(d.is_cuda() && d.is_contiguous() && (d.scalar_type() == at::kBFloat16 || d.scalar_type() == at::kFloat), "scale_grad: d");
-    CHECK_FLAT(g, d, at::kFloat);
-    TORCH_CHECK(g.numel() == 1, "scale_grad: g");
-    Guard guard(d.device());
-    if (d.numel() > 0) dpa::scale_grad(d.data_ptr(), d.scalar_type() == at::kBFloat16, g.data_ptr<float>(), d.numel(), cur_stream());
+// the gradient for an upstream gradient of `g`; `d`, if defined, holds the one for 1 and is written only where g is not
+Tensor distill_grad(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, const Tensor& g, Tensor d) {
+    dpa::DistillArgs a = distill_args(logits, ids, teacher, V, tau);
+    CHECK_FLAT(g, logits, at::kFloat);
+    TORCH_CHECK(g.numel() == 1, "distill: upstream gradient");
+    Guard guard(logits.device());
+    a.unless_one = d.defined();
+    if (!d.defined()) d = torch::empty_like(logits);
+    CHECK_FLAT16(d, logits, logits.scalar_type());
+    TORCH_CHECK(d.sizes() == logits.sizes(), "distill: gradient");
+    a.dlogits = d.data_ptr();
+    a.upstream = g.data_ptr<float>();
+    dpa::distill(a, logits.scalar_type() == at::kBFloat16, 0.f, nullptr, cur_stream());
+    return d;
 }
 // When a gradient will be asked for the forward kernel writes it beside the loss, for an upstream gradient of 1; backward
-// multiplies by the real one only when it is not 1 (tested on the device).  A second backward through the node forms it again.
+// forms it again only when the real one is not 1 (tested on the device), and so does a second backward through the node.
 struct DistillNode : public torch::autograd::Function<DistillNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool for_backward) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits_, const Tensor& ids, const Tensor& teacher, int64_t V, double tau, bool for_backward) {
+        const Tensor logits = flat16(logits_);                                 // rows lie on 16 bytes as those of the gradient do
         auto r = distill(logits, ids, teacher, V, tau, for_backward);
         if (for_backward) {
             ctx->save_for_backward({logits, ids, teacher});
@@ -356,11 +373,9 @@ struct DistillNode : public torch::autograd::Function<DistillNode> {
         if (at != ctx->saved_data.end()) {
             d = at->second.toTensor();
             ctx->saved_data.erase(at);
-        } else {
-            d = distill(s[0], s[1], s[2], ctx->saved_data["V"].toInt(), ctx->saved_data["tau"].toDouble(), true)[1];
         }
-        scale_grad(d, g[0].reshape({1}));
-        return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return {distill_grad(s[0], s[1], s[2], ctx->saved_data["V"].toInt(), ctx->saved_data["tau"].toDouble(), g[0].reshape({1}), d),
+                Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 Tensor distillation_loss(const Tensor& logits, const Tensor& ids, const Tensor& teacher, int64_t V, double tau) {

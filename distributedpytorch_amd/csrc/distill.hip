@@ -18,6 +18,9 @@
 // The teacher's p goes through LDS; its share of the gradient - at most K places of a row - is written over the dense part
 // behind a barrier, every place by all the entries that name it with the same sum, so that duplicates need neither an
 // order nor an atomic.  The loss is folded in a fixed order by a second small kernel.
+// The forward writes the gradient for an upstream gradient of 1.  Backward starts the same kernel with the real one: where that is 1
+// nothing is done, and otherwise the gradient is formed again from the logits, which crosses memory as often as scaling the
+// written one would and rounds once.
 #include <stdexcept>
 #include <string>
 #include "common.h"
@@ -163,7 +166,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     __shared__ int ids_s[KMAX];
     __shared__ float p_s[KMAX];
     const int tid = threadIdx.x;
-    const float c = a.inv_tau * LOG2E;
+    const float c = a.inv_tau * LOG2E, up = a.upstream != nullptr ? *a.upstream : 1.f, grad_scale = a.grad_scale * up;
+    if (a.unless_one && up == 1.f) return;                                     // the whole launch: the gradient is there already
     u32x4 raw[HELD], nraw[PIPE ? HELD : 1];
     Teacher<KE> te, nte;
     float total = 0.f;
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         }
         if (next < a.N) load_student((const T*)a.logits + next * a.ld, nte);
         if (r.d != nullptr) {
-            const float g = a.grad_scale * inv;
+            const float g = grad_scale * inv;
             if (any)
                 with_exponent([&](auto&& e) {
                     sweep([&](int i, float (&v)[N], bool sure) {
@@ -305,7 +309,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
                 if (te.id[i] >= 0) {
                     float same = 0.f;
                     for (int k = 0; k < a.K; ++k) same += ids_s[k] == te.id[i] ? p_s[k] : 0.f;
-                    put1(r.d + te.id[i], (fast_exp2(exponent(te.z[i])) * inv - same) * a.grad_scale);
+                    put1(r.d + te.id[i], (fast_exp2(exponent(te.z[i])) * inv - same) * grad_scale);
                 }
         if (any) total += term;
         __syncthreads();                                                       // ids_s and p_s are read
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 #pragma unroll
             for (int k = 0; k < HELD; ++k) raw[k] = nraw[k];
     }
-    if (tid == 0) a.row_loss[blockIdx.x] = total;
+    if (tid == 0 && a.row_loss != nullptr) a.row_loss[blockIdx.x] = total;
 }
 
 // loss = scale * sum of the workgroups' shares, fixed order
@@ -324,14 +328,6 @@ __global__ __launch_bounds__(256) void fold_loss_kernel(const float* __restrict_
     for (int i = threadIdx.x; i < n; i += 256) s += part[i];
     s = fold2<4, false>(s, 0.f, red).x;
     if (threadIdx.x == 0) *loss = s * scale;
-}
-
-// d *= *g unless *g is 1
-template <typename T>
-__global__ __launch_bounds__(256) void scale_grad_kernel(T* __restrict__ d, const float* __restrict__ g, long n) {
-    const float gs = *g;
-    if (gs == 1.f) return;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) put1(d + i, get1(d + i) * gs);
 }
 
 template <typename T, int NT, int NREG, bool LDS, bool PIPE, bool WHOLE>
@@ -399,14 +395,7 @@ void distill(const DistillArgs& a, int is_bf16, float loss_scale, float* loss, h
         if (is_bf16) launch<unsigned short>(a, blocks, st);
         else launch<float>(a, blocks, st);
     }
-    hipLaunchKernelGGL(fold_loss_kernel, dim3(1), dim3(256), 0, st, a.row_loss, blocks, loss_scale, loss);
-}
-
-void scale_grad(void* d, int is_bf16, const float* g, long n, hipStream_t st) {
-    long b = (n + 255) / 256;
-    const unsigned blocks = (unsigned)(b < 1 ? 1 : b > 4096 ? 4096 : b);
-    if (is_bf16) hipLaunchKernelGGL((scale_grad_kernel<unsigned short>), dim3(blocks), dim3(256), 0, st, (unsigned short*)d, g, n);
-    else hipLaunchKernelGGL((scale_grad_kernel<float>), dim3(blocks), dim3(256), 0, st, (float*)d, g, n);
+    if (loss != nullptr) hipLaunchKernelGGL(fold_loss_kernel, dim3(1), dim3(256), 0, st, a.row_loss, blocks, loss_scale, loss);
 }
 
 }  // namespace dpa

@@ -288,15 +288,16 @@ struct DistillArgs {
     void* dlogits;                         // same, or nullptr: no gradient
     const void* ids;                       // [N, K] int64 (ids64) or int32
     const float* teacher;                  // [N, K]
-    float* row_loss;                       // [distill_blocks] scratch
+    float* row_loss;                       // [distill_blocks] scratch, or nullptr: no loss
+    const float* upstream;                 // what the gradient is multiplied by, or nullptr: 1
+    int unless_one;                        // nothing is done where *upstream is 1
     long N, ld;
     int V, K, ids64;
     float inv_tau, grad_scale;             // 1 / tau, tau / N
 };
 int distill_max_entries();
 int distill_blocks(int is_bf16, long N, long ld);
-void distill(const DistillArgs& a, int is_bf16, float loss_scale /* tau^2 / N */, float* loss, hipStream_t st);
-void scale_grad(void* d, int is_bf16, const float* g, long n, hipStream_t st);   // d *= *g unless *g is 1
+void distill(const DistillArgs& a, int is_bf16, float loss_scale /* tau^2 / N */, float* loss /* or nullptr */, hipStream_t st);
 // y = addend + x * keep(seed, offset, i) / (1 - p)  (bf16, n % 8 == 0; addend optional): element dropout with the mask
 // drawn in line, fused with the residual add that follows it in a transformer block
 void dropout_bf16(const void* x, const void* addend, void* y, long n, float p, uint64_t seed, uint64_t offset, hipStream_t st);

@@ -39,8 +39,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     int32) names.  An entry is dead when its id lies outside ``[0, n_classes)`` or its logit is ``-inf`` (short lists are
     padded so); an id may come twice; a row without live entries (a prompt's) contributes zero loss and gradient.
 
-    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once, and once more by an upstream gradient other than 1), zero in the padding columns.  ``logits`` are not
-    changed.  On the GPU: bf16 or fp32 logits, fp32 teacher logits, ``K`` up to 1024.
+    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once), zero in the padding columns.  ``logits`` are not changed.  The forward
+    writes it for an upstream gradient of 1; any other (a weight beside a second loss, accumulation) costs backward one more pass over the logits.  On the GPU: bf16 or fp32 logits, fp32 teacher logits, ``K`` up to 1024.
     """
     if logits.dim() < 1 or not logits.dtype.is_floating_point:
         raise ValueError("distillation_loss: logits must be floating point [..., columns]")

@@ -593,6 +593,26 @@ def test_distillation_rows_of_the_lowest_values(V, dtype):
     _within(torch.autograd.grad(got, zd)[0], d, 2.0 ** -16 * (logq.exp() + full) / 6 + (U16 if dtype == torch.bfloat16 else U32) * d.abs() + 1e-38, "dlogits")
 
 
+@pytest.mark.parametrize("V", [700, 5000, 110000, 220000])
+@pytest.mark.parametrize("weight", [0.3, 1.0, 0.0, -7.0])
+def test_distillation_gradient_for_any_upstream_is_rounded_once(V, weight):
+    """bf16: half a step of the weighted gradient and the kernel's 2^-16, not a second half step for the weight."""
+    N, K, tau = 3, 20, 2.0
+    z = _rand(N, V, seed=V, std=2.0)
+    ids, t = _teacher(N, V, K, V)
+    live = (ids >= 0) & (ids < V) & (t > -math.inf)
+    p = torch.softmax((t.double() / tau).masked_fill(~live, -math.inf), 1) * live
+    full = torch.zeros(N, V, dtype=torch.float64).scatter_add_(1, torch.where(live, ids, 0), p)
+    q = torch.softmax(z.double() / tau, 1)
+    d = (q - full) * tau / N * weight
+    zd = z.to(DEV).requires_grad_()
+    got = ops.distillation_loss(zd, ids.to(DEV), t.to(DEV), temperature=tau)
+    g = torch.tensor(weight, device=DEV)
+    grads = [torch.autograd.grad(got, zd, g, retain_graph=True)[0] for _ in range(2)]
+    assert torch.equal(grads[0], grads[1])
+    _within(grads[0], d, 2.0 ** -16 * (q + full) * tau / N * abs(weight) + U16 * d.abs() + 1e-38, "dlogits")
+
+
 def test_distillation_gradient_against_differences():
     N, V, K, tau = 6, 300, 12, 2.0
     z = _rand(N, V, seed=3, std=2.0, dtype=torch.float32).to(DEV).requires_grad_()
