@@ -5,6 +5,7 @@
 // The nodes are C++ and not Python functions because the smallest calls are all host time: the engine runs a backward on a
 // thread of its own, and a Python node has to win the interpreter lock there first.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -353,6 +354,13 @@ Tensor distill_grad(const Tensor& logits, const Tensor& ids, const Tensor& teach
     dpa::distill(a, logits.scalar_type() == at::kBFloat16, 0.f, nullptr, cur_stream());
     return d;
 }
+// A saved tensor apart from the node's others, so that backward can let go of it while the node lives on.  Saved-tensor hooks
+// (offloading, checkpointing) see it as they see those.
+struct Kept : public torch::CustomClassHolder {
+    torch::autograd::SavedVariable t;
+    explicit Kept(const Tensor& x) : t(x, false) {}
+};
+
 // When a gradient will be asked for the forward kernel writes it beside the loss, for an upstream gradient of 1; backward
 // forms it again only when the real one is not 1 (tested on the device), and so does a second backward through the node.
 struct DistillNode : public torch::autograd::Function<DistillNode> {
@@ -361,7 +369,7 @@ struct DistillNode : public torch::autograd::Function<DistillNode> {
         auto r = distill(logits, ids, teacher, V, tau, for_backward);
         if (for_backward) {
             ctx->save_for_backward({logits, ids, teacher});
-            ctx->saved_data["V"] = V; ctx->saved_data["tau"] = tau; ctx->saved_data["d"] = r[1];
+            ctx->saved_data["V"] = V; ctx->saved_data["tau"] = tau; ctx->saved_data["d"] = at::IValue::make_capsule(c10::make_intrusive<Kept>(r[1]));
         }
         return r[0].view(at::IntArrayRef());
     }
@@ -371,8 +379,10 @@ struct DistillNode : public torch::autograd::Function<DistillNode> {
         Tensor d;
         const auto at = ctx->saved_data.find("d");
         if (at != ctx->saved_data.end()) {
-            d = at->second.toTensor();
+            d = c10::static_intrusive_pointer_cast<Kept>(at->second.toCapsule())->t.unpack();
             ctx->saved_data.erase(at);
+            // a hook kept it, or made something else of it
+            if (d.use_count() > 1 || d.storage().use_count() > 1 || !d.is_contiguous() || !on16(d)) d = Tensor();
         }
         return {distill_grad(s[0], s[1], s[2], ctx->saved_data["V"].toInt(), ctx->saved_data["tau"].toDouble(), g[0].reshape({1}), d),
                 Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};

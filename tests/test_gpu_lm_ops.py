@@ -613,6 +613,41 @@ def test_distillation_gradient_for_any_upstream_is_rounded_once(V, weight):
     _within(grads[0], d, 2.0 ** -16 * (q + full) * tau / N * abs(weight) + U16 * d.abs() + 1e-38, "dlogits")
 
 
+@pytest.mark.parametrize("weight", [1.0, 0.3])
+def test_distillation_keeps_its_gradient_where_saved_tensor_hooks_see_it(weight):
+    """Offloading moves all that the node keeps, the written gradient among it; hooks that hold on to what they were given find it
+    unchanged; a checkpoint forms it again."""
+    from torch.utils.checkpoint import checkpoint
+    N, V = 64, 4096
+    z = _rand(N, V, seed=1, std=2.0).to(DEV).requires_grad_()
+    ids, t = (x.to(DEV) for x in _teacher(N, V, 20, 1))
+    g = torch.tensor(weight, device=DEV)
+
+    def loss():
+        return ops.distillation_loss(z, ids, t, temperature=2.0)
+    (want,) = torch.autograd.grad(loss(), z, g)
+    held = []
+
+    def hold(x):
+        held.append((x, x.detach().clone()))
+        return x
+    with torch.autograd.graph.saved_tensors_hooks(hold, lambda x: x):
+        one = loss()
+    assert sum(x.shape == (N, V) for x, _ in held) == 2                            # the logits and the gradient
+    for _ in range(2):
+        assert torch.equal(torch.autograd.grad(one, z, g, retain_graph=True)[0], want)
+    assert all(torch.equal(x, y) for x, y in held)
+    held.clear()
+    del one
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        one = loss()
+    assert torch.cuda.memory_allocated() - before < N * V
+    assert torch.equal(torch.autograd.grad(one, z, g)[0], want)
+    assert torch.equal(torch.autograd.grad(checkpoint(loss, use_reentrant=False), z, g)[0], want)
+
+
 def test_distillation_gradient_against_differences():
     N, V, K, tau = 6, 300, 12, 2.0
     z = _rand(N, V, seed=3, std=2.0, dtype=torch.float32).to(DEV).requires_grad_()
