@@ -943,6 +943,7 @@ __global__ __launch_bounds__(256, 2) void attend_bwd_kv_wide_kernel(AttendArgs a
         }
 #undef DPA_FETCH_Q
     }
+    tiles_landed();                                                 // where no query sees a key nobody has waited for the values
     store_key<CAPPED>(a, o, dKt, dVt, b, key, hq0, kdoc >= 0, h);
 }
 

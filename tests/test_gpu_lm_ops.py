@@ -225,6 +225,24 @@ def test_attention_padding_holds_anything(D):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_rows_of_padding_leave_their_neighbours_alone(D):
+    """Workgroups that visit no tile end at once; those that take their place on the chip find nothing of theirs."""
+    B, T = 96, 200
+    q, k, v, do = (_rand(B, T, 2, D, seed=s).to(DEV) for s in range(4))
+    docs = torch.zeros(B, T, dtype=torch.int32, device=DEV)
+    docs[::2] = -1
+
+    def go(rows):
+        ts = [t[rows].detach().requires_grad_() for t in (q, k, v)]
+        out = ops.attention(*ts, documents=docs[rows])
+        return (out.detach(), *torch.autograd.grad(out, ts, do[rows]))
+    alone = go(slice(1, None, 2))
+    for _ in range(3):
+        for a, b in zip(go(slice(None)), alone):
+            assert torch.equal(a[1::2], b) and (a[::2] == 0).all()
+
+
 def test_attention_single_visible_key_has_no_score_gradient():
     q, k, v, do = (_rand(3, 1, 2, 128, seed=s, std=3.0).to(DEV) for s in range(4))
     leaf = [t.requires_grad_() for t in (q, k, v)]
