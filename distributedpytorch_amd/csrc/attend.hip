@@ -19,7 +19,8 @@
 //     forward in bf16, `rest`): where a few keys carry a row, dS is a small difference of dP and delta, and delta from the
 //     rounded O alone costs dQ and dK as much accuracy as their own rounding does (3.8e-3 against 2.5e-3 of the norm at
 //     scores of standard deviation 8 under a cap of 30).
-//   * Rows behind a document number < 0 are staged as zeros: whatever a padded row holds reaches no product.
+//   * Rows behind a document number < 0 are staged as zeros, so that whatever a padded row holds reaches no sum (the values that the
+//     dK / dV kernel of width 128 keeps are not: a padded key's reach its own column of dP alone, which its mask zeroes).
 //
 // Bound by the matrix cores and the vector instructions between their products (exponentials, masks, rounding), which a wave
 // does not overlap by itself.  One row of 8192, 16 query heads over 4 of width 128, with a bias: forward 347 us (790 TFLOP/s of

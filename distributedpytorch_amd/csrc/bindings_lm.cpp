@@ -228,11 +228,8 @@ struct HeadsNode : public torch::autograd::Function<HeadsNode> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once();
         const auto s = ctx->get_saved_variables();
-        const int64_t Hq = ctx->saved_data["Hq"].toInt(), Hkv = ctx->saved_data["Hkv"].toInt(), D = s[0].size(2) / (Hq + 2 * Hkv);
-        // an output that nothing used has no gradient
-        auto given = [&](const Tensor& t, int64_t h) { return t.defined() ? flat16(t) : torch::zeros({s[0].size(0), s[0].size(1), h, D}, s[0].options()); };
-        auto d = heads_bwd(s[0], Hq, Hkv, opt(s[1]), opt(s[2]), opt(s[3]), opt(s[4]), ctx->saved_data["eps"].toDouble(),
-                           ctx->saved_data["interleaved"].toBool(), given(g[0], Hq), given(g[1], Hkv), given(g[2], Hkv));
+        auto d = heads_bwd(s[0], ctx->saved_data["Hq"].toInt(), ctx->saved_data["Hkv"].toInt(), opt(s[1]), opt(s[2]), opt(s[3]), opt(s[4]),
+                           ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(), flat16(g[0]), flat16(g[1]), flat16(g[2]));
         return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };

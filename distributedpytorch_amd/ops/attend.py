@@ -63,9 +63,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     Rows that are not padding hold finite numbers: as in any product with probabilities of zero, a NaN or infinity there may
     reach queries that do not see it.
 
+    Scores are formed in fp32 and lie within 1e29 of zero; past some 1e4 their own last place shows in the probabilities.
+    Head dimensions up to 64 run in kernels of width 64 and the others in kernels of width 128: the products of the channels that
+    are not there are computed, so 32, 80 or 96 cost what 64 or 128 do.
+
     Gradients for ``q``, ``k``, ``v``; the rest are constants.  Sums, statistics and scores are fp32; probabilities and
     score gradients are rounded to bf16 for the matrix products that follow them, outputs and gradients once at the end.
-    Results do not depend on launch order.
+    Results do not depend on launch order.  On the GPU first derivatives only: a backward with ``create_graph`` is refused.
     """
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention: q, k, v must be [B, T, heads, D]")

@@ -11,7 +11,7 @@ import torch
 
 from . import _ext
 
-MAX_ENTRIES = 1024                       # teacher entries of a row on the GPU: one per thread of a workgroup
+MAX_ENTRIES = 1024                       # teacher entries of a row on the GPU: one to four per thread of a workgroup
 
 
 def _plain(logits, ids, teacher, n_classes, tau):
@@ -39,8 +39,10 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     int32) names.  An entry is dead when its id lies outside ``[0, n_classes)`` or its logit is ``-inf`` (short lists are
     padded so); an id may come twice; a row without live entries (a prompt's) contributes zero loss and gradient.
 
-    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once), zero in the padding columns.  ``logits`` are not changed.  The forward
-    writes it for an upstream gradient of 1; any other (a weight beside a second loss, accumulation) costs backward one more pass over the logits.  On the GPU: bf16 or fp32 logits, fp32 teacher logits, ``K`` up to 1024.
+    Gradient for ``logits`` (its type; fp32 arithmetic, rounded once), zero in the padding columns.  ``logits`` are not changed.
+    On the GPU: bf16 or fp32 logits, fp32 teacher logits, ``K`` up to 1024.  There the forward writes the gradient for an upstream
+    gradient of 1, and any other (a weight beside a second loss, accumulation) costs backward another pass over the logits; first
+    derivatives only: a backward with ``create_graph`` is refused.
     """
     if logits.dim() < 1 or not logits.dtype.is_floating_point:
         raise ValueError("distillation_loss: logits must be floating point [..., columns]")

@@ -41,6 +41,7 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, weight_lp: torch
 
     On the GPU ``weight [V, C]`` is the fp32 master (``C`` a multiple of 8), ``weight_lp`` its bf16 shadow (made on the fly when
     absent), the output bf16; the gradient is fp32, added into the flat gradient buffer where a sink is installed.
+    First derivatives only: without a sink a backward with ``create_graph`` is refused, into one it adds as ever.
     """
     if tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"token_embedding: tokens must be int64 or int32, got {tokens.dtype}")

@@ -56,7 +56,8 @@ def qk_norm_rotary(qkv: torch.Tensor, n_head: int, n_kv_head: Optional[int] = No
     ``0 .. T-1``) may be any whole numbers, angles are formed in 64 bits.  On the GPU: bf16, ``D`` a multiple of 8 up to 256,
     ``R`` a multiple of 16.  ``v`` is a view of ``qkv``.
 
-    Gradients for ``qkv`` and the two gains (fp32, summed in a fixed order).
+    Gradients for ``qkv`` and the two gains (fp32, summed in a fixed order); on the GPU first derivatives only: a backward with
+    ``create_graph`` is refused.
     """
     n_kv_head = n_head if n_kv_head is None else n_kv_head
     if qkv.dim() != 3 or n_head < 1 or n_kv_head < 1 or qkv.shape[2] == 0 or qkv.shape[2] % (n_head + 2 * n_kv_head):
