@@ -292,7 +292,7 @@ template <int CAPPED>
 __device__ __forceinline__ float map_score(const ScoreMap& m, float s, float& f) {
     if (CAPPED == CAP) {
         const float e = fast_exp2(s * m.k1), r = __builtin_amdgcn_rcpf(1.f + e);
-        f = r * fminf(e * r, 1.f);                                  // (an infinite e: r = 0, and the NaN gives way to 1)
+        f = r * __builtin_amdgcn_fmed3f(e * r, 0.f, 1.f);           // (the clamp rides the product; an infinite e: r = 0, and the NaN of e r becomes 0)
         return fmaf(r, -2.f * m.cap2, m.cap2);
     }
     if (CAPPED == WIDE_CAP) {
