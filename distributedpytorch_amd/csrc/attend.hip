@@ -42,7 +42,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MASKED = -2.0e30f;       // below every running maximum (which starts at NEG_BIG): exp2 gives 0 even in a row without keys
 constexpr int BQ = 128;                  // rows of a workgroup
 // The kernels' builds by cap: none, one up to CAP_MOST, a wider one (map_score).  At CAP_MOST the first form leaves a score 4.5e-5
-// off, a hundredth of what rounding P to bf16 does.
+// off, a hundredth of what rounding P to bf16 does; the wider form takes 628 us where it takes 503 (four rows of 2047, 16 heads over 4
+// of 128, forward and backward).
 constexpr int NO_CAP = 0, CAP = 1, WIDE_CAP = 2;
 constexpr float CAP_MOST = 256.f;
 
