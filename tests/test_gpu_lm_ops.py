@@ -666,6 +666,25 @@ def test_distillation_keeps_its_gradient_where_saved_tensor_hooks_see_it(weight)
     assert torch.equal(torch.autograd.grad(checkpoint(loss, use_reentrant=False), z, g)[0], want)
 
 
+@pytest.mark.parametrize("weight", [1.0, 0.3])
+def test_distillation_off_16_bytes_and_without_rows(weight):
+    """Logits that begin anywhere are copied by the call; no rows give no loss."""
+    N, V = 5, 300
+    ids, t = (x.to(DEV) for x in _teacher(N, V, 12, 2))
+    flat = _rand(N * V + 8, seed=3).to(DEV)
+    g = torch.tensor(weight, device=DEV)
+    odd = flat[1:1 + N * V].view(N, V).detach().requires_grad_()
+    assert odd.data_ptr() % 16 and odd.is_contiguous()
+    even = odd.detach().clone().requires_grad_()
+    a, b = (ops.distillation_loss(z, ids, t) for z in (odd, even))
+    assert torch.equal(a, b)
+    for _ in range(2):
+        assert torch.equal(*(torch.autograd.grad(y, z, g, retain_graph=True)[0] for y, z in ((a, odd), (b, even))))
+    none = torch.zeros(0, V, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    loss = ops.distillation_loss(none, ids[:0], t[:0])
+    assert loss.item() == 0.0 and torch.autograd.grad(loss, none, g)[0].shape == (0, V)
+
+
 def test_distillation_gradient_against_differences():
     N, V, K, tau = 6, 300, 12, 2.0
     z = _rand(N, V, seed=3, std=2.0, dtype=torch.float32).to(DEV).requires_grad_()
